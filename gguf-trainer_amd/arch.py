@@ -125,11 +125,15 @@ class Model:
             q = ag.linear(n1, L["qProj"])
             k = ag.linear(n1, L["kProj"])
             v = ag.linear(n1, L["vProj"])
-            if c.arch in ("qwen3", "gemma3"):
-                q = ag.rms_norm_heads(q, L["qNorm"], rows, c.heads, c.head_dim, c.rms_eps)
-                k = ag.rms_norm_heads(k, L["kNorm"], rows, c.kv_heads, c.head_dim, c.rms_eps)
-            q = ag.rope(q, T, c.heads, c.head_dim, rope_b)
-            k = ag.rope(k, T, c.kv_heads, c.head_dim, rope_b)
+            normed = c.arch in ("qwen3", "gemma3")
+            if normed and getattr(ag._be(), "fuse_qk_norm_rope", False):
+                q, k = ag.qk_norm_rope(q, k, L["qNorm"], L["kNorm"], T, c.heads, c.kv_heads, c.head_dim, c.rms_eps, rope_b)
+            else:
+                if normed:
+                    q = ag.rms_norm_heads(q, L["qNorm"], rows, c.heads, c.head_dim, c.rms_eps)
+                    k = ag.rms_norm_heads(k, L["kNorm"], rows, c.kv_heads, c.head_dim, c.rms_eps)
+                q = ag.rope(q, T, c.heads, c.head_dim, rope_b)
+                k = ag.rope(k, T, c.kv_heads, c.head_dim, rope_b)
             a = ag.attention(q, k, v, T, c.heads, c.kv_heads, c.head_dim, window)
             attn_out = ag.linear(a, L["oProj"])
             if c.arch == "gemma3":

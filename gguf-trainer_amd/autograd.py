@@ -353,6 +353,36 @@ def rope(x, T: int, H: int, hd: int, base: float, pos_offset: int = 0):
     return _be().rope(x, T, H, hd, base, pos_offset)
 
 
+def qk_norm_rope(q, k, q_weight, k_weight, T: int, Hq: int, Hkv: int, hd: int, eps: float, base: float, pos_offset: int = 0, positions=None):
+    """(rope(rms_norm_heads(q)), rope(rms_norm_heads(k))), the four calls of a layer with QK-norm (src/arch/qwen3.ts:153-195,
+    src/arch/gemma3.ts:173-223), as one op where the backend has it. `positions`: one integer per row instead of (row mod T) +
+    pos_offset, for rows that each belong to a sequence of their own (the composed form has no such rotation)."""
+    for t, w, H, name in ((q, q_weight, Hq, "q"), (k, k_weight, Hkv, "k")):
+        assert_matrix(t, name, "qkNormRope")
+        if t.shape[1] != H * hd or w.size != hd:
+            raise ValueError(f"qkNormRope: {name} is [{', '.join(map(str, t.shape))}] with a gain of {w.size}, expected {H} heads of {hd}")
+    if q.shape[0] != k.shape[0]:
+        raise ValueError(f"qkNormRope: q has {q.shape[0]} rows and k {k.shape[0]}")
+    rows = q.shape[0]
+    if positions is not None:
+        positions = _as_int_array(positions, "qkNormRope", "position")
+        if len(positions) != rows:
+            raise ValueError(f"qkNormRope: {len(positions)} positions for {rows} rows")
+        if len(positions) and (positions.min() < -2**31 or positions.max() >= 2**31):
+            raise ValueError("qkNormRope: a position does not fit 32 bits")
+    elif T < 1 or rows % T:
+        raise ValueError(f"qkNormRope: {rows} rows are not a whole number of sequences of {T}")
+    be = _be()
+    # one tensor in both places takes two gradients, which the one-launch backward would write at once
+    if hasattr(be, "qk_norm_rope") and q is not k and q_weight is not k_weight and hd % 2 == 0 and hd <= 1024:
+        return be.qk_norm_rope(q, k, q_weight, k_weight, T, Hq, Hkv, hd, eps, base, pos_offset, positions)
+    if positions is not None:
+        raise ValueError("qkNormRope: positions need the fused op (even head size up to 1024, q and k distinct)")
+    q = rms_norm_heads(q, q_weight, rows, Hq, hd, eps)
+    k = rms_norm_heads(k, k_weight, rows, Hkv, hd, eps)
+    return rope(q, T, Hq, hd, base, pos_offset), rope(k, T, Hkv, hd, base, pos_offset)
+
+
 def attention(q, k, v, T: int, Hq: int, Hkv: int, hd: int, window: int = 0):
     return _be().attention(q, k, v, T, Hq, Hkv, hd, window)
 

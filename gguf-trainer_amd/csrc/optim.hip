@@ -18,24 +18,9 @@
 // as one batch (see below).
 #include <algorithm>
 #include <vector>
-#include "common.h"
+#include "optim.h"
 
 typedef float v4f __attribute__((ext_vector_type(4)));
-
-#define CHUNK 2048
-
-struct Chunk { int tensor; int len; int64_t off; };
-struct TensorPtrs { float *w, *g, *m, *v; };
-
-struct gt_adamw {
-  int n = 0, nchunks = 0;
-  double total_elems = 0;
-  double beta1, beta2, eps, wd, clip;
-  Chunk *chunks = nullptr;
-  TensorPtrs *ptrs = nullptr;
-  float *partial = nullptr;     // [nchunks]
-  float *scale = nullptr;       // [2]: clip scale, grad norm
-};
 
 __global__ __launch_bounds__(256) void adamw_ssq_k(const Chunk *__restrict__ chunks, const TensorPtrs *__restrict__ ptrs,
                                                    float *__restrict__ partial) {
@@ -324,9 +309,11 @@ static int group_alloc(gt_ctx *ctx, MuonGroup &G) {
   return 0;
 }
 
-static void adamw_release(gt_adamw *o) {
+void adamw_release(gt_adamw *o) {
   if (o->chunks) (void)hipFree(o->chunks);
   if (o->ptrs) (void)hipFree(o->ptrs);
+  if (o->chunks8) (void)hipFree(o->chunks8);
+  if (o->sums8) (void)hipFree(o->sums8);
   if (o->partial) (void)hipFree(o->partial);
   if (o->scale) (void)hipFree(o->scale);
   delete o;
@@ -417,6 +404,7 @@ int gt_grad_fold(gt_ctx *ctx, int n, const gt_buf *dst, const int *dst_acc, int 
 int gt_adamw_step(gt_ctx *ctx, gt_adamw *o, double lr, double bc1, double bc2) {
   GT_ENTER(ctx);
   GT_REQUIRE(ctx, o, "gt_adamw_step: null optimizer");
+  GT_REQUIRE(ctx, !o->bits8, "gt_adamw_step: this group's states are held in 8 bits: use gt_adamw8_step");
   GT_REQUIRE(ctx, bc1 > 0 && bc2 > 0, "gt_adamw_step: bias corrections must be positive");
   if (o->nchunks == 0) return 0;
   int64_t total = 0;

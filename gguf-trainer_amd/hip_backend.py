@@ -28,7 +28,10 @@ What differs from the reference, on purpose:
     as the reference's small-T path keeps its probabilities (webgpu.ts:1176-1189).
   * Consecutive micro-batches are recorded on different streams (see __init__), each with its own pool of transient
     buffers and its own parameter-gradient accumulators, summed in stream order before anything reads them.
-  Each of these has a switch (batch_linears, fuse_residual_add, fuse_sibling_dx, group_dw, alias_add_grads, attn_keep_scores) and
+  * On request (fuse_qk_norm_rope) the per-head norms of q and k and their rotations are one op, one launch each way; the
+    normalised rows never exist in memory.
+  Each of these has a switch (batch_linears, fuse_residual_add, fuse_sibling_dx, group_dw, alias_add_grads, attn_keep_scores,
+  fuse_qk_norm_rope) and
   gives the same gradients as the one-launch-per-op form: bit for bit, or to rounding where a sum changes its order.
 """
 from __future__ import annotations
@@ -88,7 +91,8 @@ class _EntryMap:
 
 class _Entry:
     __slots__ = ("data", "grad", "nbytes", "external", "grad_init", "lazy_act", "consumers", "fused_uses",
-                 "region", "keep_grad", "extra", "needs_grad", "lazy_lin", "grad_src", "stream", "sgrad", "rope_of", "rope_fused")
+                 "region", "keep_grad", "extra", "needs_grad", "lazy_lin", "grad_src", "stream", "sgrad", "rope_of", "rope_fused",
+                 "grad_unrotated")
 
     def __init__(self, nbytes, external):
         self.data = 0
@@ -107,8 +111,9 @@ class _Entry:
         self.grad_src = 0           # another tensor's gradient buffer that holds this gradient's value so far (add's backward)
         self.stream = 0             # the stream whose launches produce and consume this tensor (its buffers come from that stream's pool)
         self.sgrad = None           # parameters: {stream: [accumulator, written?]} of the streams other than the first
-        self.rope_of = None         # a rotation's output: (input tensor, (T, hd, base, pos))
+        self.rope_of = None         # a rotation's output: (input tensor, (T, hd, base, pos)); of a norm and rotation in one: (None, ...)
         self.rope_fused = False     # an attention backward wrote the rotation's input gradient itself: the rotation's closure has nothing to do
+        self.grad_unrotated = False # an attention backward left the gradient of the rows before the rotation here
 
 
 class HipBackend:
@@ -182,6 +187,9 @@ class HipBackend:
         # attention's backward applies the backward of the rotations its q and k came through in the write-backs of dQ and
         # dK (gt_attn_bwd_scores_rope) where q / k are rotation outputs nobody else has read: no rope.bwd launch is left
         self.fuse_rope_bwd = True
+        # model graphs with QK-norm take ag.qk_norm_rope for their two norms and two rotations: fewer launches and bytes, the same
+        # gradients to rounding. Off by default, so that a run repeats the bits of earlier ones
+        self.fuse_qk_norm_rope = False
         self.fuse_residual_add = True
         # add's backward hands its upstream gradient on instead of copying it: an operand whose gradient has no writer yet
         # points at the upstream buffer (grad_src). A reader takes that buffer as it is; the first later writer adds to its
@@ -1267,6 +1275,48 @@ class HipBackend:
         out._backward = bw
         return out
 
+    def qk_norm_rope(self, q, k, qw, kw, T, Hq, Hkv, hd, eps, base, pos_offset=0, positions=None):
+        """Both head norms and both rotations as one launch, and their backward as another. The outputs are two tensors with
+        one closure: k's output names q's as its predecessor, so q's closure runs when both gradients are complete."""
+        self._op_begin(q, k, qw, kw)
+        rows = q.shape[0]
+        base, pos_offset = float(base), int(pos_offset)
+        qd, kd, qwd, kwd = self._data(q), self._data(k), self._data(qw), self._data(kw)
+        places = 0 if positions is None else self._upload(np.ascontiguousarray(positions, dtype=np.int32))
+        qo, eq = self._make_out([rows, Hq * hd], [q, k, qw, kw])
+        ko, ek = self._make_out([rows, Hkv * hd], [qo])
+        if positions is None:
+            eq.rope_of = ek.rope_of = (None, (T, hd, base, pos_offset))
+        ldq, ldk = Hq * hd, Hkv * hd
+        check(self._ctx, lib.gt_qk_norm_rope_fwd(self._ctx, rows, T, Hq, Hkv, hd, eps, base, pos_offset, places, qd, ldq, qwd, eq.data, ldq,
+                                                 kd, ldk, kwd, ek.data, ldk), "qkNormRope")
+        wants_q, wants_k = qw.requires_grad, kw.requires_grad
+
+        def bw():
+            gq, gk = self._gsrc(qo), self._gsrc(ko)
+            rq, rk = (0 if self._entries[t].grad_unrotated else 1 for t in (qo, ko))
+            dq, aq = self._gdst(q)
+            dk, ak = self._gdst(k)
+            dwq, awq = self._gdst(qw) if wants_q else (0, 0)
+            dwk, awk = self._gdst(kw) if wants_k else (0, 0)
+            nparts = C.c_int(0)
+            if self.defer_norm_dw and (dwq or dwk):
+                check(self._ctx, lib.gt_qk_norm_rope_parts_rows(self._ctx, rows, hd, C.byref(nparts)), "qkNormRope.bwd")
+            if nparts.value > 0:
+                pq, pk = (self._scratch_buf(nparts.value * hd * 4) if d else 0 for d in (dwq, dwk))
+                check(self._ctx, lib.gt_qk_norm_rope_bwd_parts(self._ctx, rows, T, Hq, Hkv, hd, eps, base, pos_offset, places, qd, ldq, qwd, gq, ldq,
+                                                               rq, dq, aq, pq, kd, ldk, kwd, gk, ldk, rk, dk, ak, pk), "qkNormRope.bwd")
+                for w, p, d, a in ((qw, pq, dwq, awq), (kw, pk, dwk, awk)):
+                    if d:
+                        self._pend_cs.append((p, nparts.value, hd, d, a))
+                        self._pend_cs_ids.add(id(w))
+                return
+            check(self._ctx, lib.gt_qk_norm_rope_bwd(self._ctx, rows, T, Hq, Hkv, hd, eps, base, pos_offset, places, qd, ldq, qwd, gq, ldq, rq, dq, aq,
+                                                     dwq, awq, kd, ldk, kwd, gk, ldk, rk, dk, ak, dwk, awk), "qkNormRope.bwd")
+
+        qo._backward = bw
+        return qo, ko
+
     def attention(self, q, k, v, T, Hq, Hkv, hd, window=0):
         self._op_begin(q, k, v)
         rows = q.shape[0]
@@ -1300,6 +1350,8 @@ class HipBackend:
             src, par = te.rope_of
             if par[0] != T or par[1] != hd:
                 return None
+            if src is None:
+                return t, par                       # its own closure does the norm's part and skips the rotation's
             se = self._entries.get(src)
             if se is None or (se.external and not src.requires_grad):
                 return None
@@ -1315,10 +1367,11 @@ class HipBackend:
                 dq, aq = self._gdst(rq[0] if rq else q)
                 dk, ak = self._gdst(rk[0] if rk else k)
                 dv, av = self._gdst(v)
-                if rq:
-                    self._entries[q].rope_fused = True
-                if rk:
-                    self._entries[k].rope_fused = True
+                for t, r in ((q, rq), (k, rk)):
+                    if r and r[0] is t:
+                        self._entries[t].grad_unrotated = True
+                    elif r:
+                        self._entries[t].rope_fused = True
                 check(self._ctx, lib.gt_attn_bwd_scores_rope(self._ctx, B, T, Hq, Hkv, hd, window, qd, kd, vd, od, g, lse, scores,
                                                              par[2], par[3], 1 if rq else 0, 1 if rk else 0,
                                                              dq, aq, dk, ak, dv, av), "attention.bwd")
@@ -1438,12 +1491,14 @@ def init_hip(device: int = 0, streams: int = 4):
         return None
 
 
-def require_gpu(purpose: str, device: int = 0, streams: int = 4, bf16_pieces: bool = False) -> HipBackend:
+def require_gpu(purpose: str, device: int = 0, streams: int = 4, bf16_pieces: bool = False, fuse_qk_norm_rope: bool = False) -> HipBackend:
     """requireGPU analogue (webgpu.ts:1812). bf16_pieces: run the FP32 products and the attention kernels that have such a form on
     the bf16 matrix instruction (library options "gemm.split_bf16" and "attn.split_bf16": each FP32 element as three exact bf16
-    pieces, FP32 accumulation; as close to float64 as the FP32 MFMA kernels, about 1.3 x faster steps, not bit-identical to them)."""
+    pieces, FP32 accumulation; as close to float64 as the FP32 MFMA kernels, about 1.3 x faster steps, not bit-identical to them). fuse_qk_norm_rope: the norms and rotations of q and k in models with
+    QK-norm as one op (HipBackend.qk_norm_rope)."""
     try:
         gpu = HipBackend(device, streams)
+        gpu.fuse_qk_norm_rope = fuse_qk_norm_rope
         if bf16_pieces:
             gpu.set_option("gemm.split_bf16", 1)
             gpu.set_option("attn.split_bf16", 1)

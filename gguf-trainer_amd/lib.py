@@ -74,6 +74,12 @@ _SIG = {
     "gt_embedding_bwd": [ctxp, i32, i32, i32, buf, buf, buf, i32],
     "gt_rope": [ctxp, i32, i32, i32, i32, f64, i32, i32, buf, buf, i32],
     "gt_rope_pair": [ctxp, i32, i32, i32, f64, i32, i32, i32, buf, buf, i32, i32, buf, buf, i32],
+    "gt_qk_norm_rope_fwd": [ctxp, i32, i32, i32, i32, i32, f32, f64, i32, buf, buf, i64, buf, buf, i64, buf, i64, buf, buf, i64],
+    "gt_qk_norm_rope_bwd": [ctxp, i32, i32, i32, i32, i32, f32, f64, i32, buf, buf, i64, buf, buf, i64, i32, buf, i32, buf, i32,
+                            buf, i64, buf, buf, i64, i32, buf, i32, buf, i32],
+    "gt_qk_norm_rope_parts_rows": [ctxp, i32, i32, C.POINTER(i32)],
+    "gt_qk_norm_rope_bwd_parts": [ctxp, i32, i32, i32, i32, i32, f32, f64, i32, buf, buf, i64, buf, buf, i64, i32, buf, i32, buf,
+                                  buf, i64, buf, buf, i64, i32, buf, i32, buf],
     "gt_attn_fwd": [ctxp, i32, i32, i32, i32, i32, i32, buf, buf, buf, buf, buf],
     "gt_attn_bwd": [ctxp, i32, i32, i32, i32, i32, i32, buf, buf, buf, buf, buf, buf, buf, i32, buf, i32, buf, i32],
     "gt_gemm_add": [ctxp, i32, i32, i32, i32, buf, buf, buf, buf],
@@ -95,6 +101,11 @@ _SIG = {
     "gt_adamw_step": [ctxp, C.c_void_p, f64, f64, f64],
     "gt_adamw_grad_norm": [ctxp, C.c_void_p, C.POINTER(f32)],
     "gt_adamw_destroy": [ctxp, C.c_void_p],
+    "gt_adamw8_create": [ctxp, i32, C.POINTER(buf), C.POINTER(buf), C.POINTER(buf), C.POINTER(buf), C.POINTER(buf), C.POINTER(i64),
+                         f64, f64, f64, f64, f64, C.POINTER(C.c_void_p)],
+    "gt_adamw8_step": [ctxp, C.c_void_p, f64, f64, f64, C.c_uint64],
+    "gt_adamw8_read": [ctxp, C.c_void_p, i32, buf, buf],
+    "gt_adamw8_write": [ctxp, C.c_void_p, i32, buf, buf],
     "gt_muon_create": [ctxp, i32, C.POINTER(buf), C.POINTER(buf), C.POINTER(buf), C.POINTER(i32), C.POINTER(i32),
                        f64, i32, i32, C.POINTER(C.c_void_p)],
     "gt_muon_step": [ctxp, C.c_void_p, f64],

@@ -19,26 +19,43 @@ def _bufs(vals):
     return (c_buf * len(vals))(*vals)
 
 
+_BLOCK8 = 256            # elements that share the exponents of their two 8-bit moments
+
+
 class AdamWHip:
-    def __init__(self, gpu, params, lr, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.0, clip=1.0):
+    """state_bits = 8 holds the moments as e4m3 values with an exponent per 256 elements (gt_adamw8_create in include/ggufhip.h): 2 bytes
+    of state per parameter instead of 8. The step number is the seed of the random rounding, and exported state is FP32 and
+    comes back unchanged, so a resumed run repeats an uninterrupted one."""
+
+    def __init__(self, gpu, params, lr, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.0, clip=1.0, state_bits=32):
+        if state_bits not in (8, 32):
+            raise ValueError(f"AdamW: state_bits must be 8 or 32, got {state_bits}")
+        self.state_bits = state_bits
         self.gpu = gpu
         self.params = list(params)
         self.base_lr = lr
         self.lr_scale = 1.0
         self.beta1, self.beta2, self.eps, self.weight_decay, self.clip = beta1, beta2, eps, weight_decay, clip
         self.t = 0
-        self._m, self._v = [], []
+        self._m, self._v, self._e = [], [], []
         w, g = [], []
+        per = 1 if state_bits == 8 else 4
         for p in self.params:
             b = gpu.buffers_for(p)          # uploads host weights once; accumulator on the device
             gpu.keep_grad_on_device(p)
             w.append(b["data"])
             g.append(b["grad"])
-            self._m.append(gpu.create_state_buffer(p.size * 4))
-            self._v.append(gpu.create_state_buffer(p.size * 4))
+            self._m.append(gpu.create_state_buffer(p.size * per))
+            self._v.append(gpu.create_state_buffer(p.size * per))
+            if state_bits == 8:
+                self._e.append(gpu.create_state_buffer(2 * (-(-p.size // _BLOCK8))))
         self._h = C.c_void_p()
         n = len(self.params)
         sizes = (C.c_int64 * max(1, n))(*[p.size for p in self.params])
+        if state_bits == 8:
+            check(gpu.ctx, lib.gt_adamw8_create(gpu.ctx, n, _bufs(w), _bufs(g), _bufs(self._m), _bufs(self._v), _bufs(self._e), sizes,
+                                                beta1, beta2, eps, weight_decay, clip, C.byref(self._h)), "gt_adamw8_create")
+            return
         check(gpu.ctx, lib.gt_adamw_create(gpu.ctx, n, _bufs(w), _bufs(g), _bufs(self._m), _bufs(self._v), sizes,
                                            beta1, beta2, eps, weight_decay, clip, C.byref(self._h)), "gt_adamw_create")
 
@@ -48,14 +65,14 @@ class AdamWHip:
     def destroy(self):
         """Release the device-side tables; the moment buffers go back with the backend's state buffers."""
         if self.gpu._destroyed:             # the library context is gone and took the tables and the buffers with it
-            self._h, self._m, self._v = C.c_void_p(), [], []
+            self._h, self._m, self._v, self._e = C.c_void_p(), [], [], []
             return
         if self._h:
             check(self.gpu.ctx, lib.gt_adamw_destroy(self.gpu.ctx, self._h), "gt_adamw_destroy")
             self._h = C.c_void_p()
-        for b in self._m + self._v:
+        for b in self._m + self._v + self._e:
             self.gpu.free_state_buffer(b)
-        self._m, self._v = [], []
+        self._m, self._v, self._e = [], [], []
 
     def zero_grad(self):
         """No-op: accumulators live on the device and are re-armed when a step has consumed them."""
@@ -65,7 +82,11 @@ class AdamWHip:
         bc1 = 1 - self.beta1 ** self.t
         bc2 = 1 - self.beta2 ** self.t
         self.gpu.ensure_grads_defined(self.params)
-        check(self.gpu.ctx, lib.gt_adamw_step(self.gpu.ctx, self._h, self.base_lr * self.lr_scale, bc1, bc2), "gt_adamw_step")
+        lr = self.base_lr * self.lr_scale
+        if self.state_bits == 8:
+            check(self.gpu.ctx, lib.gt_adamw8_step(self.gpu.ctx, self._h, lr, bc1, bc2, self.t), "gt_adamw8_step")
+        else:
+            check(self.gpu.ctx, lib.gt_adamw_step(self.gpu.ctx, self._h, lr, bc1, bc2), "gt_adamw_step")
         self.gpu.grads_consumed(self.params)
 
     def grad_norm(self) -> float:
@@ -77,13 +98,41 @@ class AdamWHip:
         for p in self.params:
             p.data[:] = self.gpu.read_state_buffer(self.gpu.buffers_for(p)["data"], p.size)
 
+    def _moment_pair(self):
+        """Two FP32 buffers that hold the moments of any one tensor of the group on their way in or out."""
+        n = 4 * max((p.size for p in self.params), default=0)
+        return self.gpu.create_state_buffer(n), self.gpu.create_state_buffer(n)
+
     def export_state(self):
+        if self.state_bits == 8:
+            out = {"m": [], "v": [], "t": self.t}
+            bm, bv = self._moment_pair()
+            for i, p in enumerate(self.params):
+                check(self.gpu.ctx, lib.gt_adamw8_read(self.gpu.ctx, self._h, i, bm, bv), "gt_adamw8_read")
+                out["m"].append(self.gpu.read_state_buffer(bm, p.size))
+                out["v"].append(self.gpu.read_state_buffer(bv, p.size))
+            self.gpu.free_state_buffer(bm)
+            self.gpu.free_state_buffer(bv)
+            return out
         return {"m": [self.gpu.read_state_buffer(b, p.size) for b, p in zip(self._m, self.params)],
                 "v": [self.gpu.read_state_buffer(b, p.size) for b, p in zip(self._v, self.params)], "t": self.t}
 
     def import_state(self, s):
         if len(s["m"]) != len(self.params) or len(s["v"]) != len(self.params):
             raise ValueError(f"adam state count mismatch: {len(s['m'])}/{len(s['v'])} vs {len(self.params)}")
+        if self.state_bits == 8:
+            for p, m, v in zip(self.params, s["m"], s["v"]):
+                if np.asarray(m).size != p.size or np.asarray(v).size != p.size:
+                    raise ValueError(f"adam state size mismatch: {np.asarray(m).size}/{np.asarray(v).size} vs {p.size}")
+            bm, bv = self._moment_pair()
+            for i, (m, v) in enumerate(zip(s["m"], s["v"])):
+                self.gpu.write_state_buffer(bm, np.asarray(m, dtype=np.float32))
+                self.gpu.write_state_buffer(bv, np.asarray(v, dtype=np.float32))
+                check(self.gpu.ctx, lib.gt_adamw8_write(self.gpu.ctx, self._h, i, bm, bv), "gt_adamw8_write")
+            self.gpu.free_state_buffer(bm)
+            self.gpu.free_state_buffer(bv)
+            self.t = int(s["t"])
+            return
         for b, a in zip(self._m, s["m"]):
             self.gpu.write_state_buffer(b, np.asarray(a, dtype=np.float32))
         for b, a in zip(self._v, s["v"]):

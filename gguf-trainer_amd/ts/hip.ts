@@ -79,6 +79,10 @@ const SYMBOLS = {
   gt_embedding_fwd:      { parameters: [ptr, i32, i32, i32, u64, u64, u64], result: i32 },
   gt_embedding_bwd:      { parameters: [ptr, i32, i32, i32, u64, u64, u64, i32], result: i32 },
   gt_rope:               { parameters: [ptr, i32, i32, i32, i32, f64, i32, i32, u64, u64, i32], result: i32 },
+  gt_qk_norm_rope_fwd:   { parameters: [ptr, i32, i32, i32, i32, i32, f32, f64, i32, u64, u64, i64, u64, u64, i64, u64, i64, u64, u64, i64], result: i32 },
+  gt_qk_norm_rope_bwd:   { parameters: [ptr, i32, i32, i32, i32, i32, f32, f64, i32, u64, u64, i64, u64, u64, i64, i32, u64, i32, u64, i32, u64, i64, u64, u64, i64, i32, u64, i32, u64, i32], result: i32 },
+  gt_qk_norm_rope_parts_rows: { parameters: [ptr, i32, i32, buf], result: i32 },
+  gt_qk_norm_rope_bwd_parts: { parameters: [ptr, i32, i32, i32, i32, i32, f32, f64, i32, u64, u64, i64, u64, u64, i64, i32, u64, i32, u64, u64, i64, u64, u64, i64, i32, u64, i32, u64], result: i32 },
   gt_rope_pair:          { parameters: [ptr, i32, i32, i32, f64, i32, i32, i32, u64, u64, i32, i32, u64, u64, i32], result: i32 },
   gt_attn_fwd:           { parameters: [ptr, i32, i32, i32, i32, i32, i32, u64, u64, u64, u64, u64], result: i32 },
   gt_attn_bwd:           { parameters: [ptr, i32, i32, i32, i32, i32, i32, u64, u64, u64, u64, u64, u64, u64, i32, u64, i32, u64, i32], result: i32 },
@@ -95,6 +99,10 @@ const SYMBOLS = {
   gt_soft_ce_bwd:        { parameters: [ptr, i32, i32, i32, u64, u64, u64, f32, u64, u64, f32, u64, i32], result: i32 },
   gt_grad_fold:          { parameters: [ptr, i32, buf, buf, i32, buf, buf], result: i32 },
   gt_adamw_create:       { parameters: [ptr, i32, buf, buf, buf, buf, buf, f64, f64, f64, f64, f64, buf], result: i32 },
+  gt_adamw8_create:      { parameters: [ptr, i32, buf, buf, buf, buf, buf, buf, f64, f64, f64, f64, f64, buf], result: i32 },
+  gt_adamw8_step:        { parameters: [ptr, ptr, f64, f64, f64, u64], result: i32 },
+  gt_adamw8_read:        { parameters: [ptr, ptr, i32, u64, u64], result: i32 },
+  gt_adamw8_write:       { parameters: [ptr, ptr, i32, u64, u64], result: i32 },
   gt_adamw_step:         { parameters: [ptr, ptr, f64, f64, f64], result: i32 },
   gt_adamw_grad_norm:    { parameters: [ptr, ptr, buf], result: i32 },
   gt_adamw_destroy:      { parameters: [ptr, ptr], result: i32 },
@@ -752,6 +760,37 @@ export class HipBackend implements OpsBackend, RegionBackend {
     return out;
   }
 
+  /** rope(rmsNormHeads(q)) and rope(rmsNormHeads(k)) as one launch each way (gt_qk_norm_rope_*), for a host whose layer bodies
+   * (src/arch/qwen3.ts, gemma3.ts) call it in place of the four ops. k's output names q's as its predecessor, so the closure
+   * on q's output runs when both gradients are complete. q and k, and their gains, must be distinct tensors. */
+  qkNormRope(
+    q: Tensor, k: Tensor, qw: Tensor, kw: Tensor, T: number, Hq: number, Hkv: number, hd: number, eps: number, base: number,
+    posOffset: number,
+  ): [Tensor, Tensor] {
+    if (q === k || qw === kw) throw new Error("qkNormRope: q and k, and their gains, must be distinct tensors");
+    const rows = q.shape[0], ldq = BigInt(Hq * hd), ldk = BigInt(Hkv * hd);
+    const qd = this.dataOf(q), kd = this.dataOf(k), qwd = this.dataOf(qw), kwd = this.dataOf(kw);
+    const { t: qo, e: eq } = this.makeOut([rows, Hq * hd], [q, k, qw, kw]);
+    const { t: ko, e: ek } = this.makeOut([rows, Hkv * hd], [qo]);
+    this.check(
+      this.sym.gt_qk_norm_rope_fwd(this.ctx, rows, T, Hq, Hkv, hd, eps, base, posOffset, 0n, qd, ldq, qwd, eq.data, ldq, kd, ldk, kwd, ek.data, ldk),
+      "qkNormRope",
+    );
+    const wantsQ = qw.requiresGrad, wantsK = kw.requiresGrad;
+    qo._backward = () => {
+      const gq = this.gradOf(qo), gk = this.gradOf(ko);
+      const [dq, aq] = this.gradDst(q), [dk, ak] = this.gradDst(k);
+      const [dwq, awq] = wantsQ ? this.gradDst(qw) : [0n, 0] as [DevBuf, number];
+      const [dwk, awk] = wantsK ? this.gradDst(kw) : [0n, 0] as [DevBuf, number];
+      this.check(
+        this.sym.gt_qk_norm_rope_bwd(this.ctx, rows, T, Hq, Hkv, hd, eps, base, posOffset, 0n, qd, ldq, qwd, gq, ldq, 1, dq, aq, dwq, awq,
+          kd, ldk, kwd, gk, ldk, 1, dk, ak, dwk, awk),
+        "qkNormRope.bwd",
+      );
+    };
+    return [qo, ko];
+  }
+
   attention(q: Tensor, k: Tensor, v: Tensor, T: number, Hq: number, Hkv: number, hd: number, window: number): Tensor {
     const rows = q.shape[0];
     if (rows % T) throw new Error(`attention: ${rows} rows are not a whole number of sequences of ${T}`);
@@ -884,41 +923,57 @@ export class HipBackend implements OpsBackend, RegionBackend {
 // ---- optimizers ---------------------------------------------------------------------------------------------------------
 const u64s = (v: DevBuf[]) => BigUint64Array.from(v.length ? v : [0n]);
 
+/** AdamOpts and how the moments are held: in FP32, or (8) as e4m3 values with an exponent per 256 elements (gt_adamw8_create). */
+export interface AdamHipOpts extends AdamOpts {
+  stateBits?: 8 | 32; // default 32
+}
+
 /** AdamWGpu (adamw-gpu.ts:131-251) over gt_adamw_*: weights, gradients and moments stay on the device; a step is three
- * launches for any number of tensors (sum of squares, clip scale, fused update). */
+ * launches for any number of tensors (sum of squares, clip scale, fused update; two with 8-bit moments). */
 export class AdamWHip {
   readonly params: Tensor[];
   private gpu: HipBackend;
-  private opts: Required<AdamOpts>;
+  private opts: Required<AdamHipOpts>;
   private baseLr: number;
   private lrScale = 1;
   private t = 0;
   private handle: Deno.PointerValue = null;
   private mBufs: DevBuf[] = [];
   private vBufs: DevBuf[] = [];
+  private eBufs: DevBuf[] = []; // 8-bit moments: the exponents of each tensor's blocks
 
-  constructor(gpu: HipBackend, params: Tensor[], opts: AdamOpts) {
+  constructor(gpu: HipBackend, params: Tensor[], opts: AdamHipOpts) {
     this.gpu = gpu;
     this.params = params;
-    this.opts = { beta1: 0.9, beta2: 0.999, eps: 1e-8, weightDecay: 0.0, clip: 1.0, ...opts };
+    this.opts = { beta1: 0.9, beta2: 0.999, eps: 1e-8, weightDecay: 0.0, clip: 1.0, stateBits: 32, ...opts };
     this.baseLr = opts.lr;
+    const per = this.opts.stateBits === 8 ? 1 : 4;
     const w: DevBuf[] = [], g: DevBuf[] = [];
     for (const p of params) {
       const b = gpu.buffersFor(p); // uploads host weights once; accumulator on the device
       gpu.keepGradOnDevice(p);
       w.push(b.data);
       g.push(b.grad);
-      this.mBufs.push(gpu.createStateBuffer(p.size * 4));
-      this.vBufs.push(gpu.createStateBuffer(p.size * 4));
+      this.mBufs.push(gpu.createStateBuffer(p.size * per));
+      this.vBufs.push(gpu.createStateBuffer(p.size * per));
+      if (this.opts.stateBits === 8) this.eBufs.push(gpu.createStateBuffer(2 * Math.ceil(p.size / 256)));
     }
     const sizes = BigInt64Array.from(params.length ? params.map((p) => BigInt(p.size)) : [0n]);
     const out = new BigUint64Array(1);
     const o = this.opts;
-    gpu.check(
-      gpu.symbols.gt_adamw_create(gpu.context, params.length, u64s(w), u64s(g), u64s(this.mBufs), u64s(this.vBufs), sizes,
-        o.beta1, o.beta2, o.eps, o.weightDecay, o.clip, out),
-      "gt_adamw_create",
-    );
+    if (o.stateBits === 8) {
+      gpu.check(
+        gpu.symbols.gt_adamw8_create(gpu.context, params.length, u64s(w), u64s(g), u64s(this.mBufs), u64s(this.vBufs), u64s(this.eBufs),
+          sizes, o.beta1, o.beta2, o.eps, o.weightDecay, o.clip, out),
+        "gt_adamw8_create",
+      );
+    } else {
+      gpu.check(
+        gpu.symbols.gt_adamw_create(gpu.context, params.length, u64s(w), u64s(g), u64s(this.mBufs), u64s(this.vBufs), sizes,
+          o.beta1, o.beta2, o.eps, o.weightDecay, o.clip, out),
+        "gt_adamw_create",
+      );
+    }
     this.handle = Deno.UnsafePointer.create(out[0]);
   }
   setLrScale(scale: number) {
@@ -931,7 +986,13 @@ export class AdamWHip {
     const o = this.opts;
     const bc1 = 1 - Math.pow(o.beta1, this.t), bc2 = 1 - Math.pow(o.beta2, this.t);
     this.gpu.ensureGradsDefined(this.params);
-    this.gpu.check(this.gpu.symbols.gt_adamw_step(this.gpu.context, this.handle, this.baseLr * this.lrScale, bc1, bc2), "gt_adamw_step");
+    const lr = this.baseLr * this.lrScale;
+    if (o.stateBits === 8) { // the step number seeds the random rounding
+      const seed = BigInt(this.t);
+      this.gpu.check(this.gpu.symbols.gt_adamw8_step(this.gpu.context, this.handle, lr, bc1, bc2, seed), "gt_adamw8_step");
+    } else {
+      this.gpu.check(this.gpu.symbols.gt_adamw_step(this.gpu.context, this.handle, lr, bc1, bc2), "gt_adamw_step");
+    }
     this.gpu.gradsConsumed(this.params);
   }
   /** ||g|| of the last step (what the clip compared with its threshold). */
@@ -943,8 +1004,24 @@ export class AdamWHip {
   async syncWeightsToHost(): Promise<void> {
     await this.gpu.sync(this.params);
   }
+  /** Two FP32 buffers that hold the moments of any one tensor of the group on their way in or out. */
+  private momentPair(): [DevBuf, DevBuf] {
+    const n = 4 * this.params.reduce((a, p) => Math.max(a, p.size), 0);
+    return [this.gpu.createStateBuffer(n), this.gpu.createStateBuffer(n)];
+  }
   async exportState(): Promise<{ m: Float32Array[]; v: Float32Array[]; t: number }> {
     const m: Float32Array[] = [], v: Float32Array[] = [];
+    if (this.opts.stateBits === 8) {
+      const [bm, bv] = this.momentPair();
+      for (let i = 0; i < this.params.length; i++) {
+        this.gpu.check(this.gpu.symbols.gt_adamw8_read(this.gpu.context, this.handle, i, bm, bv), "gt_adamw8_read");
+        m.push(await this.gpu.readStateBuffer(bm, this.params[i].size));
+        v.push(await this.gpu.readStateBuffer(bv, this.params[i].size));
+      }
+      this.gpu.freeStateBuffer(bm);
+      this.gpu.freeStateBuffer(bv);
+      return { m, v, t: this.t };
+    }
     for (let i = 0; i < this.params.length; i++) {
       m.push(await this.gpu.readStateBuffer(this.mBufs[i], this.params[i].size));
       v.push(await this.gpu.readStateBuffer(this.vBufs[i], this.params[i].size));
@@ -955,6 +1032,23 @@ export class AdamWHip {
     if (s.m.length !== this.params.length || s.v.length !== this.params.length) {
       throw new Error(`adam state count mismatch: ${s.m.length}/${s.v.length} vs ${this.params.length}`);
     }
+    if (this.opts.stateBits === 8) {
+      for (let i = 0; i < this.params.length; i++) {
+        if (s.m[i].length !== this.params[i].size || s.v[i].length !== this.params[i].size) {
+          throw new Error(`adam state size mismatch: ${s.m[i].length}/${s.v[i].length} vs ${this.params[i].size}`);
+        }
+      }
+      const [bm, bv] = this.momentPair();
+      for (let i = 0; i < this.params.length; i++) {
+        this.gpu.writeStateBuffer(bm, s.m[i]);
+        this.gpu.writeStateBuffer(bv, s.v[i]);
+        this.gpu.check(this.gpu.symbols.gt_adamw8_write(this.gpu.context, this.handle, i, bm, bv), "gt_adamw8_write");
+      }
+      this.gpu.freeStateBuffer(bm);
+      this.gpu.freeStateBuffer(bv);
+      this.t = s.t;
+      return;
+    }
     for (let i = 0; i < this.params.length; i++) {
       this.gpu.writeStateBuffer(this.mBufs[i], s.m[i]);
       this.gpu.writeStateBuffer(this.vBufs[i], s.v[i]);
@@ -964,15 +1058,15 @@ export class AdamWHip {
   destroy() {
     if (this.gpu.isDestroyed) { // the context took the tables and the buffers with it
       this.handle = null;
-      this.mBufs = this.vBufs = [];
+      this.mBufs = this.vBufs = this.eBufs = [];
       return;
     }
     if (this.handle) {
       this.gpu.check(this.gpu.symbols.gt_adamw_destroy(this.gpu.context, this.handle), "gt_adamw_destroy");
       this.handle = null;
     }
-    for (const b of [...this.mBufs, ...this.vBufs]) this.gpu.freeStateBuffer(b);
-    this.mBufs = this.vBufs = [];
+    for (const b of [...this.mBufs, ...this.vBufs, ...this.eBufs]) this.gpu.freeStateBuffer(b);
+    this.mBufs = this.vBufs = this.eBufs = [];
   }
 }
 
@@ -981,7 +1075,7 @@ export interface MuonHipOpts {
   momentum?: number; // default 0.95
   nesterov?: boolean; // default true
   nsSteps?: number; // Newton-Schulz iterations, default 5
-  aux: AdamOpts; // AdamW settings for the non-Muon group
+  aux: AdamHipOpts; // AdamW settings for the non-Muon group
 }
 
 /** MuonGpu (muon-gpu.ts:351-470) over gt_muon_*: matrices of equal shape are stepped as one batch. */

@@ -230,6 +230,33 @@ int gt_rope(gt_ctx *ctx, int rows, int T, int H, int hd, double base, int pos, i
 int gt_rope_pair(gt_ctx *ctx, int rows, int T, int hd, double base, int pos, int backward, int H1, gt_buf in1, gt_buf out1, int acc1,
                  int H2, gt_buf in2, gt_buf out2, int acc2);
 
+/* ---- QK-norm and RoPE in one pass: rmsNormHeads on q and k (webgpu.ts:1085-1088) and rope on both results (:1110-1121), as
+ * src/arch/qwen3.ts and gemma3.ts compose them: four dispatches there, one here, each way.
+ * Rows are tokens; q has Hq heads of hd elements per row, k has Hkv. Every head is divided by its root mean square and multiplied by
+ * the gain wq (wk) [hd], then its pairs (j, j + hd/2) are turned by position * base^(-2j/hd). The position of row r is (r mod T) + pos;
+ * with `places` (an int32 device buffer of `rows` entries, any values) it is places[r], T and pos are not read, and the rows may
+ * belong to as many sequences as there are rows (one new token of each). Angles are formed in 64 bits.
+ * Strides are in elements between consecutive rows: ldq / ldk of q / k and of dq / dk, ldqo / ldko of the rotated rows and ldgq / ldgk
+ * of their gradients; a row's heads lie next to each other, so q and k may be slices of one wider product. qo may be q itself
+ * and ko k itself (same stride). hd is even and at most 1024; multiples of 8 up to 512 with 16-byte aligned buffers and strides of
+ * whole 16-byte chunks take the vector kernels, everything else a generic one.
+ * Backward: q and k are the rows before the norm (nothing is kept from the forward). rot_q (rot_k) = 1: gq (gk) is the gradient of
+ * the rotated rows; 0: of the rows between norm and rotation, what gt_attn_bwd_scores_rope leaves. A destination of 0 (dq, dk, dwq,
+ * dwk) is skipped. dq (dk) may be gq (gk) itself where strides agree and acc is 0. Results do not depend on timing.
+ * The gain sums go through the context's workspace; gt_qk_norm_rope_bwd_parts instead leaves gt_qk_norm_rope_parts_rows partial rows
+ * of hd floats per side in the caller's buffers (0: that side's sums are not wanted), for gt_colsum_group to add when they are
+ * needed: the same bits, and no allocation under a graph capture. */
+int gt_qk_norm_rope_fwd(gt_ctx *ctx, int rows, int T, int Hq, int Hkv, int hd, float eps, double base, int pos, gt_buf places,
+                        gt_buf q, int64_t ldq, gt_buf wq, gt_buf qo, int64_t ldqo,
+                        gt_buf k, int64_t ldk, gt_buf wk, gt_buf ko, int64_t ldko);
+int gt_qk_norm_rope_bwd(gt_ctx *ctx, int rows, int T, int Hq, int Hkv, int hd, float eps, double base, int pos, gt_buf places,
+                        gt_buf q, int64_t ldq, gt_buf wq, gt_buf gq, int64_t ldgq, int rot_q, gt_buf dq, int acc_q, gt_buf dwq, int acc_wq,
+                        gt_buf k, int64_t ldk, gt_buf wk, gt_buf gk, int64_t ldgk, int rot_k, gt_buf dk, int acc_k, gt_buf dwk, int acc_wk);
+int gt_qk_norm_rope_parts_rows(gt_ctx *ctx, int rows, int hd, int *nparts);
+int gt_qk_norm_rope_bwd_parts(gt_ctx *ctx, int rows, int T, int Hq, int Hkv, int hd, float eps, double base, int pos, gt_buf places,
+                              gt_buf q, int64_t ldq, gt_buf wq, gt_buf gq, int64_t ldgq, int rot_q, gt_buf dq, int acc_q, gt_buf parts_q,
+                              gt_buf k, int64_t ldk, gt_buf wk, gt_buf gk, int64_t ldgk, int rot_k, gt_buf dk, int acc_k, gt_buf parts_k);
+
 /* ---- attention: srcAttnFwd / BwdD / BwdDq / BwdDkv (wgsl.ts:657-918), webgpu.ts:1142-1189 -----
  * q[B*T, Hq*hd], k,v[B*T, Hkv*hd], causal, window > 0 keeps keys [t-window+1, t]; GQA head h reads
  * kv head h / (Hq/Hkv). lse[B*Hq*T] is the saved softmax statistic (log2 domain). */
@@ -301,6 +328,24 @@ int gt_adamw_create(gt_ctx *ctx, int n, const gt_buf *w, const gt_buf *g, const 
 int gt_adamw_step(gt_ctx *ctx, gt_adamw *opt, double lr, double bc1, double bc2);
 int gt_adamw_grad_norm(gt_ctx *ctx, gt_adamw *opt, float *norm);   /* last step's global norm; waits */
 int gt_adamw_destroy(gt_ctx *ctx, gt_adamw *opt);
+
+/* The same step with the moments held in 8 bits: 2 bytes of state per parameter instead of 8, 16 (20 with the clip) bytes moved per
+ * parameter and step instead of 28 (32). No counterpart in the reference. m[i] and r[i] are sizes[i] bytes each: the first moment
+ * and the ROOT of the second as OCP e4m3 values; e[i] holds two signed bytes for each block of 256 elements (2 * ceil(sizes[i] / 256)
+ * bytes, 2-byte aligned), the exponents of m and of r: a state is its e4m3 value times 2^e. All bytes zero = zero moments. The
+ * caller owns and clears the buffers. Each step rounds the new moments up or down at random in proportion, from bits that `seed`,
+ * the block and the place in it determine: pass another seed each step (the step number will do); the same seed gives the
+ * same bits. Gradients and weights are FP32, the update uses the moments before they are rounded, and the norm for the
+ * clip is summed in 64 bits. A moment that is not finite is held as NaN. The handle is gt_adamw's: gt_adamw_grad_norm and
+ * gt_adamw_destroy take it, gt_adamw_step does not. With the clip and without it a step allocates nothing and can be captured.
+ *   gt_adamw8_read:  the moments of tensor i as FP32 values, m and v = r^2 (0: not wanted)
+ *   gt_adamw8_write: the states of tensor i from FP32 moments, rounded to nearest; what gt_adamw8_read gave comes back unchanged */
+int gt_adamw8_create(gt_ctx *ctx, int n, const gt_buf *w, const gt_buf *g, const gt_buf *m, const gt_buf *r, const gt_buf *e,
+                     const int64_t *sizes, double beta1, double beta2, double eps, double weight_decay, double clip,
+                     gt_adamw **out);
+int gt_adamw8_step(gt_ctx *ctx, gt_adamw *opt, double lr, double bc1, double bc2, uint64_t seed);
+int gt_adamw8_read(gt_ctx *ctx, gt_adamw *opt, int i, gt_buf m, gt_buf v);
+int gt_adamw8_write(gt_ctx *ctx, gt_adamw *opt, int i, gt_buf m, gt_buf v);
 
 /* dst[i] (+)= src[i*nsrc + 0] + src[i*nsrc + 1] + ... (a source of 0 is skipped), i < n, sizes[i] elements each, one
  * launch for the whole list: parameter-gradient accumulators that micro-batches recorded on different streams kept
