@@ -12,13 +12,15 @@
 // two-thousandth (b2 = 0.999) of what separates it from its target, far less than half of e4m3's steps of 6 to 12 percent:
 // rounded to nearest both would stay where they are. The random bits of an element are a function of the step's seed, the
 // number of its block in the group and its place in the block, 16 for each moment, so a step repeats bit for bit. An r that
-// is there is never rounded to zero: m / (0 + eps) would follow.
-// The update itself uses m and v before they are rounded. A moment that is not finite is held as e4m3's NaN and its
-// neighbours' exponent goes by the finite ones.
+// is there is never rounded to zero: m / (0 + eps) would follow. r is unbiased, so v = r^2 is high by r's variance: where v still
+// grows by small steps up to 6 percent, half of that in the update's denominator.
+// The update itself uses m and v before they are rounded. A moment that is not finite is held as e4m3's NaN (its weight is
+// not finite either) and its neighbours' exponent goes by the finite ones.
 //
 // Bound by memory: 16 bytes per element (g read, w read and written, two codes each way), 20 with the clip, whose norm has
 // to be known before the first update. One wavefront to a block, four neighbouring elements to a lane, so that the block's
-// largest moments are one exchange within the wavefront and no LDS is used.
+// largest moments are one exchange within the wavefront and no LDS is used. About 60 vector operations per element: at
+// twice that (library roots and divisions, float comparisons for the block's largest) they were as long as the memory's time.
 #include <algorithm>
 #include "optim.h"
 
@@ -26,10 +28,18 @@ typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v2f __attribute__((ext_vector_type(2)));
 
 #define BLK8 256
-#define CHUNK8 4096                              // 16 blocks, four to a wavefront
-#define SSQ8_MAX_GROUPS 4096
+#define CHUNK8 1024                              // four blocks, one to a wavefront
+#define NORM8_PER_CU 8                           // workgroups of the norm's kernel
+#define NORM8_GROUPS 2048
+#define FOLD8_CHUNKS 2048                        // up to here the update's workgroups add up the norm's sums themselves
+// The chunk table's pointers come out of memory, where the compiler cannot see that they are global: without this its loads
+// take the flat path, which also waits for LDS.
+#define GLOBAL __attribute__((address_space(1)))
+typedef GLOBAL float gfloat;
+typedef GLOBAL v4f gv4f;
+typedef GLOBAL unsigned char gbyte;
 
-struct Adam8H { float b1, b2, omb1, omb2, eps, wd, lr, ibc1, ibc2; unsigned key; };
+struct Adam8H { float b1, b2, omb1, omb2, eps, wd, lr, ibc1, rbc2; unsigned key; };
 
 __host__ __device__ __forceinline__ unsigned mix1(unsigned x) {
   x ^= x >> 16;
@@ -42,120 +52,118 @@ __host__ __device__ __forceinline__ unsigned mix2(unsigned x) {
 }
 
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }
-// smallest e >= -126 with top <= 448 * 2^e (448 = 0.875 * 2^9)
-__device__ __forceinline__ int exponent_for(float top) {
-  if (!(top > 0.f)) return -126;
-  return max(__builtin_amdgcn_frexp_expf(top) - (__builtin_amdgcn_frexp_mantf(top) <= 0.875f ? 9 : 8), -126);
-}
-// code of y in [0, 448] (not finite: the NaN code): the lower e4m3 neighbour, or the upper one where the remainder plus
-// r16 / 65536 of a step makes a step
-__device__ __forceinline__ unsigned encode8(float y, unsigned r16) {
-  const unsigned normal = min(((__float_as_uint(y) + (r16 << 4)) >> 20) - (120u << 3), 0x7fu);
-  const unsigned small = (unsigned)(y * 512.f + (float)r16 * (1.f / 65536.f));
-  return y < 0.015625f ? small : normal;
-}
-__device__ __forceinline__ bool is_finite(float x) { return fabsf(x) <= 3.40282347e38f; }
 
-// Codes and exponents of a block's moments from their values, four elements to a lane (elements past the tensor's end as
-// zeros). bits: 16 random bits for m below 16 for r.
-__device__ __forceinline__ void encode_block(const float (&m)[4], const float (&v)[4], const unsigned (&bits)[4], unsigned &mc, unsigned &rc,
-                                             int &em, int &er) {
-  float tm = 0.f, tv = 0.f;
+// The bits of a positive float with its leading one at bit 23, and the exponent that goes with them (denormals too).
+__device__ __forceinline__ void normal_bits(unsigned b, int &e, unsigned &frac) {
+  const int sh = b >> 23 ? 0 : __builtin_clz(b | 1u) - 8;
+  e = sh ? 1 - sh : (int)(b >> 23);
+  frac = (b << sh) & 0x7fffffu;
+}
+// smallest e >= -126 with top <= 448 * 2^e, 448 = 1.75 * 2^8; whole numbers only, so that it runs on the scalar unit
+__device__ __forceinline__ int exponent_m(unsigned top) {
+  int e;
+  unsigned frac;
+  normal_bits(top, e, frac);
+  return top ? max(e - 127 - (frac <= 0x600000u ? 8 : 7), -126) : -126;
+}
+// the same for sqrt(top): top <= 448^2 * 4^e, 448^2 = 1.53125 * 2^17
+__device__ __forceinline__ int exponent_r(unsigned top) {
+  int e;
+  unsigned frac;
+  normal_bits(top, e, frac);
+  return top ? (e - 127 - (frac <= 0x440000u ? 17 : 16) + 1) >> 1 : -126;
+}
+
+// Largest of one word over the wavefront, as a scalar: four exchanges within each row of 16 lanes, the four rows on the
+// scalar unit.
+template <int CTRL> __device__ __forceinline__ unsigned dpp_max(unsigned v) {
+  const unsigned o = (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+  return v > o ? v : o;
+}
+__device__ __forceinline__ unsigned wave_umax(unsigned v) {
+  v = dpp_max<0xB1>(v);                          // neighbours
+  v = dpp_max<0x4E>(v);                          // pairs
+  v = dpp_max<0x141>(v);                         // halves of a row
+  v = dpp_max<0x140>(v);                         // rows mirrored
+  const unsigned a = __builtin_amdgcn_readlane((int)v, 0), b = __builtin_amdgcn_readlane((int)v, 16), c = __builtin_amdgcn_readlane((int)v, 32),
+                 d = __builtin_amdgcn_readlane((int)v, 48);
+  return max(max(a, b), max(c, d));
+}
+
+// sqrt(v) to the last bit or next to it: the hardware's 1 / sqrt and one Newton step. Zero stays zero, infinity and NaN give NaN; below
+// 2^-126 the result is small, but not zero.
+__device__ __forceinline__ float root(float v) {
+  const float y = __builtin_amdgcn_rsqf(__builtin_amdgcn_fmed3f(v, 1.17549435e-38f, __builtin_inff()));
+  const float s = v * y;
+  return __builtin_fmaf(__builtin_fmaf(-s, s, v), 0.5f * y, s);
+}
+
+#define FINITE_BITS 0x7f800000u                  // bits of a finite magnitude are below this
+
+// Four codes, one to a byte, from the magnitudes of four values scaled so that e4m3's exponent is theirs: y = |value| * 2^(-e - 120). A y
+// below 2^-126 is then a denormal exactly where e4m3's are, so one addition rounds both: the code is the y's bits from 20
+// up, after 16 random bits are added to the 20 below them. `low` is the least y of each (its bits), NaN and infinity
+// become the code 0x7f. The codes come back in the top seven bits but one of each word, for the caller to set the sign and gather.
+__device__ __forceinline__ unsigned code_word(float y, unsigned low, unsigned bits, unsigned place) {
+  const unsigned r = __builtin_amdgcn_perm(0u, bits, place);                 // the 16 random bits at 8..23
+  const unsigned b = min(max(__float_as_uint(y), low), 0x07f00000u);
+  return (b << 4) + r;
+}
+__device__ __forceinline__ unsigned gather(const unsigned (&t)[4]) {
+  const unsigned lo = __builtin_amdgcn_perm(t[1], t[0], 0x0c0c0703u), hi = __builtin_amdgcn_perm(t[3], t[2], 0x07030c0cu);
+  return lo | hi;
+}
+
+// Codes and exponents of a block's moments from their values and roots, four elements to a lane (elements past the tensor's
+// end as zeros). bits: 16 random bits for m below 16 for r.
+__device__ __forceinline__ void encode_block(const float (&m)[4], const float (&v)[4], const float (&r)[4], const unsigned (&bits)[4], unsigned &mc,
+                                             unsigned &rc, int &em, int &er) {
+  // magnitudes order as their bits do
+  unsigned am[4], av[4];
 #pragma unroll
-  for (int j = 0; j < 4; j++) { tm = fmaxf(tm, fabsf(m[j])); tv = fmaxf(tv, v[j]); }      // NaN drops out
-  tm = wave_max(tm);
-  tv = wave_max(tv);
-  if (!is_finite(tm) || !is_finite(tv)) {
-    tm = tv = 0.f;
+  for (int j = 0; j < 4; j++) { am[j] = __float_as_uint(m[j]) & 0x7fffffffu; av[j] = __float_as_uint(v[j]) & 0x7fffffffu; }
+  unsigned tm = wave_umax(max(max(am[0], am[1]), max(am[2], am[3])));
+  unsigned tv = wave_umax(max(max(av[0], av[1]), max(av[2], av[3])));
+  if (max(tm, tv) >= FINITE_BITS) {              // an infinity or a NaN: the exponents go by what is finite
+    tm = tv = 0;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      if (is_finite(m[j])) tm = fmaxf(tm, fabsf(m[j]));
-      if (is_finite(v[j])) tv = fmaxf(tv, v[j]);
+      if (am[j] < FINITE_BITS) tm = max(tm, am[j]);
+      if (av[j] < FINITE_BITS) tv = max(tv, av[j]);
     }
-    tm = wave_max(tm);
-    tv = wave_max(tv);
+    tm = wave_umax(tm);
+    tv = wave_umax(tv);
   }
-  em = exponent_for(tm);
-  er = exponent_for(sqrtf(tv));
-  const float sm = pow2(-em), sr = pow2(-er);
-  mc = rc = 0;
+  em = exponent_m(tm);
+  er = exponent_r(tv);
+  unsigned cm[4], cr[4];
 #pragma unroll
   for (int j = 0; j < 4; j++) {
-    const unsigned cm = encode8(fabsf(m[j]) * sm, bits[j] & 0xffffu) | (__float_as_uint(m[j]) >> 31 << 7);
-    const unsigned cr = max(encode8(sqrtf(v[j]) * sr, bits[j] >> 16), v[j] > 0.f ? 1u : 0u);
-    mc |= cm << (8 * j);
-    rc |= cr << (8 * j);
+    const unsigned c = code_word(__builtin_ldexpf(__builtin_fabsf(m[j]), -120 - em), 0u, bits[j], 0x0c01000cu);
+    cm[j] = (c & 0x7fffffffu) | (__float_as_uint(m[j]) & 0x80000000u);
+    cr[j] = code_word(__builtin_ldexpf(r[j], -120 - er), v[j] > 0.f ? 1u << 20 : 0u, bits[j], 0x0c03020cu);
   }
+  mc = gather(cm);
+  rc = gather(cr);
 }
 __device__ __forceinline__ void decode4(unsigned c, float s, float (&out)[4]) {
   const v2f lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, true);
   out[0] = lo[0] * s; out[1] = lo[1] * s; out[2] = hi[0] * s; out[3] = hi[1] * s;
 }
 // four neighbouring bytes of a block of n elements; zeros past its end
-__device__ __forceinline__ unsigned load_codes(const unsigned char *p, int i0, int n, bool whole) {
-  if (whole) return *reinterpret_cast<const unsigned *>(p + i0);
+__device__ __forceinline__ unsigned load_codes(const gbyte *p, int i0, int n, bool whole) {
+  if (whole) return __builtin_nontemporal_load((const GLOBAL unsigned *)(p + i0));
   unsigned c = 0;
 #pragma unroll
   for (int j = 0; j < 4; j++) if (i0 + j < n) c |= (unsigned)p[i0 + j] << (8 * j);
   return c;
 }
-__device__ __forceinline__ void store_codes(unsigned char *p, int i0, int n, bool whole, unsigned c) {
-  if (whole) { *reinterpret_cast<unsigned *>(p + i0) = c; return; }
+__device__ __forceinline__ void store_codes(gbyte *p, int i0, int n, bool whole, unsigned c) {
+  if (whole) { __builtin_nontemporal_store(c, (GLOBAL unsigned *)(p + i0)); return; }
 #pragma unroll
   for (int j = 0; j < 4; j++) if (i0 + j < n) p[i0 + j] = (unsigned char)(c >> (8 * j));
 }
 
-__global__ __launch_bounds__(256) void adamw8_update_k(const Chunk8 *__restrict__ chunks, const float *__restrict__ scale, Adam8H h) {
-#pragma clang fp contract(off)                   // every product is rounded before it is added: the moments are defined to the bit
-  const Chunk8 c = chunks[blockIdx.x];
-  const float sc = scale[0];
-  const int lane = threadIdx.x % WAVE, i0 = lane * 4;
-  const bool aligned = ((reinterpret_cast<uintptr_t>(c.w) | reinterpret_cast<uintptr_t>(c.g)) % 16 |
-                        (reinterpret_cast<uintptr_t>(c.m) | reinterpret_cast<uintptr_t>(c.r)) % 4) == 0;
-  for (int b = threadIdx.x / WAVE; b * BLK8 < c.len; b += 4) {
-    const int n = min(BLK8, c.len - b * BLK8);
-    const bool whole = aligned && n == BLK8;
-    float *w = c.w + b * BLK8;
-    const float *g = c.g + b * BLK8;
-    unsigned char *mp = c.m + b * BLK8, *rp = c.r + b * BLK8;
-    float gg[4] = {0, 0, 0, 0}, ww[4] = {0, 0, 0, 0}, m[4], v[4];
-    if (whole) {
-      const v4f a = reinterpret_cast<const v4f *>(g)[lane], d = reinterpret_cast<const v4f *>(w)[lane];
-#pragma unroll
-      for (int j = 0; j < 4; j++) { gg[j] = a[j]; ww[j] = d[j]; }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; j++) if (i0 + j < n) { gg[j] = g[i0 + j]; ww[j] = w[i0 + j]; }
-    }
-    decode4(load_codes(mp, i0, n, whole), pow2(c.e[2 * b]), m);
-    decode4(load_codes(rp, i0, n, whole), pow2(c.e[2 * b + 1]), v);
-    const unsigned key = mix2((c.block + b) ^ h.key);
-    unsigned bits[4];
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const float x = gg[j] * sc;
-      m[j] = m[j] * h.b1 + x * h.omb1;
-      v[j] = (v[j] * v[j]) * h.b2 + (x * h.omb2) * x;
-      float upd = (m[j] * h.ibc1) / (sqrtf(v[j] * h.ibc2) + h.eps);
-      if (h.wd > 0.f) upd += h.wd * ww[j];
-      ww[j] -= h.lr * upd;
-      bits[j] = mix1(key + (unsigned)(i0 + j) * 0x9E3779B9u);
-    }
-    unsigned mc, rc;
-    int em, er;
-    encode_block(m, v, bits, mc, rc, em, er);
-    if (whole) reinterpret_cast<v4f *>(w)[lane] = v4f{ww[0], ww[1], ww[2], ww[3]};
-    else
-#pragma unroll
-      for (int j = 0; j < 4; j++) if (i0 + j < n) w[i0 + j] = ww[j];
-    store_codes(mp, i0, n, whole, mc);
-    store_codes(rp, i0, n, whole, rc);
-    if (lane == 0) *reinterpret_cast<unsigned short *>(c.e + 2 * b) = (unsigned short)((unsigned)(em & 0xff) | (unsigned)(er & 0xff) << 8);
-  }
-}
-
-// Sum of squares of every gradient in 64 bits: each workgroup its chunks, its sum to sums[workgroup]; the workgroup that
-// comes last adds the sums in workgroup order and turns the norm into the clip scale. sums[SSQ8_MAX_GROUPS] counts.
 __device__ __forceinline__ double wave_sum64(double v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, WAVE);
@@ -168,38 +176,112 @@ __device__ __forceinline__ double block_sum64(double v, double *sm) {
   __syncthreads();
   return (sm[0] + sm[1]) + (sm[2] + sm[3]);
 }
-__global__ __launch_bounds__(256) void adamw8_norm_k(const Chunk8 *__restrict__ chunks, int nchunks, double *sums, double clip, float *scale) {
-  __shared__ double sm[4];
-  __shared__ int last;
-  double s = 0;
-  for (int k = blockIdx.x; k < nchunks; k += gridDim.x) {
-    const float *g = chunks[k].g;
-    const int len = chunks[k].len;
-    const int n4 = reinterpret_cast<uintptr_t>(g) % 16 == 0 ? len / 4 : 0;
-    for (int i = threadIdx.x; i < n4; i += 256) {
-      const v4f x = reinterpret_cast<const v4f *>(g)[i];
-#pragma unroll
-      for (int j = 0; j < 4; j++) s = fma((double)x[j], (double)x[j], s);
-    }
-    for (int i = n4 * 4 + threadIdx.x; i < len; i += 256) s = fma((double)g[i], (double)g[i], s);
-  }
-  s = block_sum64(s, sm);
-  unsigned *count = reinterpret_cast<unsigned *>(sums + SSQ8_MAX_GROUPS);
-  if (threadIdx.x == 0) {
-    __hip_atomic_store(sums + blockIdx.x, s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    last = __hip_atomic_fetch_add(count, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
-  }
-  __syncthreads();
-  if (!last) return;
+
+// The clip scale and the norm from the partial sums, in every thread of a workgroup.
+__device__ __forceinline__ float clip_scale(const double *__restrict__ sums, int nsums, double clip, double *sm, double &norm) {
   double t = 0;
-  for (unsigned i = threadIdx.x; i < gridDim.x; i += 256) t += __hip_atomic_load(sums + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  t = block_sum64(t, sm);
-  if (threadIdx.x == 0) {
-    const double norm = sqrt(t);
-    scale[0] = norm > clip ? (float)(clip / (norm + 1e-12)) : 1.0f;
-    scale[1] = (float)norm;
-    __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  for (int i = threadIdx.x; i < nsums; i += 256) t += sums[i];
+  norm = sqrt(block_sum64(t, sm));
+  return norm > clip ? (float)(clip / (norm + 1e-12)) : 1.0f;
+}
+
+// A workgroup takes one chunk, a wavefront one block, and nothing is repeated: 1642 us for 642M parameters (6.26 TB/s, a large copy
+// reaches 4.8 to 5.0 there), against 1770 with two blocks to a wavefront, 1848 with four and 2060 with as many workgroups as
+// the card holds going through all chunks. Every array is touched once a step, so all accesses are streaming ones: 1956
+// without (four blocks). nsums > 0: the clip scale is formed here from the partial sums instead of by adamw8_scale_k.
+__global__ __launch_bounds__(256) void adamw8_update_k(const Chunk8 *__restrict__ chunks, const double *__restrict__ sums, int nsums, double clip,
+                                                       float *__restrict__ scale, Adam8H h) {
+#pragma clang fp contract(off)                   // m and v: every product is rounded before it is added, so that they are defined to the bit
+  __shared__ double sm[4];
+  float sc;
+  if (nsums) {
+    double norm;
+    sc = clip_scale(sums, nsums, clip, sm, norm);
+    if (blockIdx.x == 0 && threadIdx.x == 0) { scale[0] = sc; scale[1] = (float)norm; }
+  } else {
+    sc = scale[0];
   }
+  const Chunk8 c = chunks[blockIdx.x];
+  const int lane = threadIdx.x % WAVE, i0 = lane * 4, b = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+  const int n = min(BLK8, c.len - b * BLK8);
+  if (n <= 0) return;
+  const bool whole = n == BLK8 && ((reinterpret_cast<uintptr_t>(c.w) | reinterpret_cast<uintptr_t>(c.g)) % 16 |
+                                   (reinterpret_cast<uintptr_t>(c.m) | reinterpret_cast<uintptr_t>(c.r)) % 4) == 0;
+  gfloat *w = (gfloat *)c.w + b * BLK8;
+  const gfloat *g = (const gfloat *)c.g + b * BLK8;
+  gbyte *mp = (gbyte *)c.m + b * BLK8, *rp = (gbyte *)c.r + b * BLK8;
+  GLOBAL signed char *e = (GLOBAL signed char *)c.e + 2 * b;
+  float gg[4] = {0, 0, 0, 0}, ww[4] = {0, 0, 0, 0}, m[4], v[4], r[4];
+  if (whole) {
+    const v4f a = __builtin_nontemporal_load((const gv4f *)g + lane), d = __builtin_nontemporal_load((const gv4f *)w + lane);
+#pragma unroll
+    for (int j = 0; j < 4; j++) { gg[j] = a[j]; ww[j] = d[j]; }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; j++) if (i0 + j < n) { gg[j] = g[i0 + j]; ww[j] = w[i0 + j]; }
+  }
+  decode4(load_codes(mp, i0, n, whole), pow2(e[0]), m);
+  decode4(load_codes(rp, i0, n, whole), pow2(e[1]), v);
+  const unsigned key = mix2((c.block + b) ^ h.key) + (unsigned)i0 * 0x9E3779B9u;
+  unsigned bits[4];
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const float x = gg[j] * sc;
+    m[j] = m[j] * h.b1 + x * h.omb1;
+    v[j] = (v[j] * v[j]) * h.b2 + (x * h.omb2) * x;
+    r[j] = root(v[j]);
+    // 1 / x to the last bit but one: the update is a small part of the weight
+    float upd = (m[j] * h.ibc1) * __builtin_amdgcn_rcpf(__builtin_fmaf(r[j], h.rbc2, h.eps));
+    if (h.wd > 0.f) upd = __builtin_fmaf(h.wd, ww[j], upd);
+    ww[j] = __builtin_fmaf(-h.lr, upd, ww[j]);
+    bits[j] = mix1(key + (unsigned)j * 0x9E3779B9u);
+  }
+  unsigned mc, rc;
+  int em, er;
+  encode_block(m, v, r, bits, mc, rc, em, er);
+  if (whole) __builtin_nontemporal_store(v4f{ww[0], ww[1], ww[2], ww[3]}, (gv4f *)w + lane);
+  else
+#pragma unroll
+    for (int j = 0; j < 4; j++) if (i0 + j < n) w[i0 + j] = ww[j];
+  store_codes(mp, i0, n, whole, mc);
+  store_codes(rp, i0, n, whole, rc);
+  if (lane == 0) *(GLOBAL unsigned short *)e = (unsigned short)((unsigned)(em & 0xff) | (unsigned)(er & 0xff) << 8);
+}
+
+// Sum of squares of every gradient in 64 bits: each workgroup its chunks in order, its sum to sums[workgroup]. 135M gradients in 84 us
+// (6.4 TB/s) with eight workgroups to a CU, 120 with four, 187 with two.
+__global__ __launch_bounds__(256) void adamw8_norm_k(const Chunk8 *__restrict__ chunks, int nchunks, double *__restrict__ sums) {
+  __shared__ double sm[4];
+  double s[4] = {0, 0, 0, 0};
+  // four chunks at a time, so that each thread has four loads in flight
+  for (int k = blockIdx.x * 4; k < nchunks; k += gridDim.x * 4) {
+    bool all = k + 4 <= nchunks;
+    for (int u = 0; u < 4 && all; u++) all = chunks[k + u].len == CHUNK8 && (uintptr_t)chunks[k + u].g % 16 == 0;
+    if (all) {
+      v4f x[4];
+#pragma unroll
+      for (int u = 0; u < 4; u++) x[u] = __builtin_nontemporal_load((const gv4f *)chunks[k + u].g + threadIdx.x);
+#pragma unroll
+      for (int u = 0; u < 4; u++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) s[j] = fma((double)x[u][j], (double)x[u][j], s[j]);
+      continue;
+    }
+    for (int u = k; u < min(k + 4, nchunks); u++) {
+      const gfloat *g = (const gfloat *)chunks[u].g;
+      const int len = chunks[u].len;
+      for (int i = threadIdx.x; i < len; i += 256) s[0] = fma((double)g[i], (double)g[i], s[0]);
+    }
+  }
+  const double t = block_sum64((s[0] + s[1]) + (s[2] + s[3]), sm);
+  if (threadIdx.x == 0) sums[blockIdx.x] = t;
+}
+
+__global__ __launch_bounds__(256) void adamw8_scale_k(const double *__restrict__ sums, int nsums, double clip, float *__restrict__ scale) {
+  __shared__ double sm[4];
+  double norm;
+  const float sc = clip_scale(sums, nsums, clip, sm, norm);
+  if (threadIdx.x == 0) { scale[0] = sc; scale[1] = (float)norm; }
 }
 
 // The moments of one tensor as FP32 values, and states from such values, rounded to the nearest (ties away from zero).
@@ -219,15 +301,17 @@ __global__ __launch_bounds__(256) void state8_write_k(int64_t size, unsigned cha
   const int64_t nb = (size + BLK8 - 1) / BLK8;
   for (int64_t b = (int64_t)blockIdx.x * 4 + threadIdx.x / WAVE; b < nb; b += (int64_t)gridDim.x * 4) {
     const int n = (int)min((int64_t)BLK8, size - b * BLK8);
-    float mm[4] = {0, 0, 0, 0}, vv[4] = {0, 0, 0, 0};
+    float mm[4] = {0, 0, 0, 0}, vv[4] = {0, 0, 0, 0}, rr[4];
     const unsigned half[4] = {0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
 #pragma unroll
     for (int j = 0; j < 4; j++) if (i0 + j < n) { mm[j] = m[b * BLK8 + i0 + j]; vv[j] = v[b * BLK8 + i0 + j]; }
+#pragma unroll
+    for (int j = 0; j < 4; j++) rr[j] = root(vv[j]);
     unsigned mc, rc;
     int em, er;
-    encode_block(mm, vv, half, mc, rc, em, er);
-    store_codes(mp + b * BLK8, i0, n, false, mc);
-    store_codes(rp + b * BLK8, i0, n, false, rc);
+    encode_block(mm, vv, rr, half, mc, rc, em, er);
+    store_codes((gbyte *)mp + b * BLK8, i0, n, false, mc);
+    store_codes((gbyte *)rp + b * BLK8, i0, n, false, rc);
     if (lane == 0) { e[2 * b] = (signed char)em; e[2 * b + 1] = (signed char)er; }
   }
 }
@@ -263,13 +347,11 @@ int gt_adamw8_create(gt_ctx *ctx, int n, const gt_buf *w, const gt_buf *g, const
     }
   }
   o->nchunks = (int)ch.size();
-  const std::vector<double> zero(SSQ8_MAX_GROUPS + 1, 0.0);
   const float one[2] = {1.0f, 0.0f};
   hipError_t err;
   if ((err = hipMalloc((void **)&o->chunks8, std::max<size_t>(1, ch.size()) * sizeof(Chunk8))) != hipSuccess ||
-      (err = hipMalloc((void **)&o->sums8, zero.size() * 8)) != hipSuccess || (err = hipMalloc((void **)&o->scale, 8)) != hipSuccess ||
+      (err = hipMalloc((void **)&o->sums8, NORM8_GROUPS * sizeof(double))) != hipSuccess || (err = hipMalloc((void **)&o->scale, 8)) != hipSuccess ||
       (!ch.empty() && (err = hipMemcpy(o->chunks8, ch.data(), ch.size() * sizeof(Chunk8), hipMemcpyHostToDevice)) != hipSuccess) ||
-      (err = hipMemcpy(o->sums8, zero.data(), zero.size() * 8, hipMemcpyHostToDevice)) != hipSuccess ||
       (err = hipMemcpy(o->scale, one, 8, hipMemcpyHostToDevice)) != hipSuccess) {
     (void)hipGetLastError();
     adamw_release(o);
@@ -287,15 +369,22 @@ int gt_adamw8_step(gt_ctx *ctx, gt_adamw *o, double lr, double bc1, double bc2, 
   GT_REQUIRE(ctx, bc1 > 0 && bc2 > 0, "gt_adamw8_step: bias corrections must be positive");
   if (o->nchunks == 0) return 0;
   ProfScope ps(ctx, "adamw8", o->total_elems * (o->clip > 0 ? 20.0 : 16.0));
-  if (o->clip > 0) {
-    const int nb = (int)std::min<int64_t>({o->nchunks, (int64_t)ctx->num_cu * 8, SSQ8_MAX_GROUPS});
-    hipLaunchKernelGGL(adamw8_norm_k, dim3((unsigned)nb), dim3(256), 0, ctx->stream, o->chunks8, o->nchunks, o->sums8, o->clip, o->scale);
+  const int nsums = o->clip > 0 ? (int)std::min<int64_t>({cdiv(o->nchunks, 4), (int64_t)ctx->num_cu * NORM8_PER_CU, NORM8_GROUPS}) : 0;
+  // While the update's workgroups fit the card at once each adds up the few KB of sums itself, which saves a launch: 61 chunks take
+  // 11.9 us a step this way and 14.5 the other, 4770 chunks 26 both ways, 131000 chunks 685 against 467.
+  const bool fold = o->nchunks <= FOLD8_CHUNKS;
+  if (nsums) {
+    hipLaunchKernelGGL(adamw8_norm_k, dim3((unsigned)nsums), dim3(256), 0, ctx->stream, o->chunks8, o->nchunks, o->sums8);
     GT_LAUNCHED(ctx);
   }
   // every constant is formed in f64 and rounded to f32 once
   Adam8H h{(float)o->beta1, (float)o->beta2, (float)(1.0 - o->beta1), (float)(1.0 - o->beta2), (float)o->eps, (float)o->wd,
-           (float)lr, (float)(1.0 / bc1), (float)(1.0 / bc2), mix2((unsigned)seed ^ mix2((unsigned)(seed >> 32) + 0x9E3779B9u))};
-  hipLaunchKernelGGL(adamw8_update_k, dim3((unsigned)o->nchunks), dim3(256), 0, ctx->stream, o->chunks8, o->scale, h);
+           (float)lr, (float)(1.0 / bc1), (float)(1.0 / sqrt(bc2)), mix2((unsigned)seed ^ mix2((unsigned)(seed >> 32) + 0x9E3779B9u))};
+  if (nsums && !fold) {
+    hipLaunchKernelGGL(adamw8_scale_k, dim3(1), dim3(256), 0, ctx->stream, o->sums8, nsums, o->clip, o->scale);
+    GT_LAUNCHED(ctx);
+  }
+  hipLaunchKernelGGL(adamw8_update_k, dim3((unsigned)o->nchunks), dim3(256), 0, ctx->stream, o->chunks8, o->sums8, fold ? nsums : 0, o->clip, o->scale, h);
   GT_LAUNCHED(ctx);
   return 0;
 }

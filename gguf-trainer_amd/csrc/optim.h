@@ -22,7 +22,7 @@ struct gt_adamw {
   float *scale = nullptr;       // [2]: clip scale, grad norm
   bool bits8 = false;
   Chunk8 *chunks8 = nullptr;
-  double *sums8 = nullptr;      // partial sums of squares, then the count of workgroups that have left theirs
+  double *sums8 = nullptr;      // partial sums of squares, one per workgroup of the norm's kernel
   std::vector<Tensor8> tensors8;
 };
 
