@@ -6,14 +6,16 @@
 //   backward  gy = R^T g (or g, where the rotation has been undone already);  S = sum(gy w x);
 //             dx = r w gy - x r^3 S / hd;  dw = sum over rows and heads of gy x r                        (h = hd / 2)
 //
-// Bound by memory: 8 bytes per element forward, 12 backward, about 20 operations. A head is handled by LPH lanes of one
-// wavefront, each holding four elements of the lower half and the four of the upper half they are rotated with, so a pair
-// never leaves its lane and the row sums are the only exchange. r is formed again in the backward (its row is in registers
-// anyway) instead of being stored.
+// Bound by memory: 8 bytes per element forward, 12 backward, about 20 operations. 16384 rows of 16 + 8 heads of 128 take 65.6 us
+// forward (6.1 TB/s) and 98 us backward (6.2 TB/s; the gain sums are another launch of 4 us); a large copy reaches 5.0.
+// A head is handled by LPH lanes of one wavefront, each holding four elements of the lower half and the four of the upper half
+// they are rotated with, so a pair never leaves its lane and the row sums are the only exchange. r is formed again in the
+// backward (its row is in registers anyway) instead of being stored. Every row is read once and far from its next use: all
+// accesses are streaming ones.
 //
-// The angle of pair j at position p is p * base^(-2j/hd). One thread per (row, pair) of the workgroup's rows forms it in
-// 64 bits, as a fraction of a turn with the whole turns taken off, and leaves cos and sin in LDS for every head of the row:
-// positions may be anything (a decoding batch's rows each have their own) and no table grows with them.
+// The angle of pair j at position p is p * base^(-2j/hd). One thread per pair of the workgroup's rows forms it in 64 bits, as a
+// fraction of a turn with the whole turns taken off, and leaves cos and sin in LDS for every head of the row: positions may
+// be anything (a decoding batch's rows each have their own) and no table grows with them.
 #include <algorithm>
 #include "common.h"
 
@@ -21,6 +23,14 @@ typedef float v4f __attribute__((ext_vector_type(4)));
 
 #define QK_MAX_HD 1024                           // the generic kernels keep a head's gain sums in LDS, one copy per wavefront
 #define QK_VEC_HD 512                            // 64 lanes of eight elements
+// Measured on 16384 rows of 16 + 8 heads of 128 and of 10 + 2 heads of 64 (and 32768 rows of the former, backward):
+//   forward: 4 to 6 passes (one row of the first) 65.6 and 19.5 us, 12 passes 68.5 and 20.3, 24 passes 71.2 and 20.1
+//   backward, workgroups to a CU: 2: 102.7 (197) us, 3: 104.9 (206), 4: 109 (213), 8: 113 (218), 1: 122 (263). More of them read in
+//   less of an order; loading a head ahead of its turn made it 111 (210) for the same reason. 12 passes: 33.3 us for heads of 64, 8: 36.3, 16: 35.6
+#define QK_FWD_PASSES 6
+#define QK_BWD_PASSES 12
+#define QK_BWD_PER_CU 2
+#define QK_ANGLES 1024                           // pairs of a workgroup's rows whose cosines and sines LDS holds
 
 struct QkSide {
   const float *x, *w, *g, *old;                  // rows before the norm, gain, (backward) gradient, what dx is added to
@@ -42,149 +52,181 @@ struct QkArgs {
 __device__ __forceinline__ double turns_per_place(double log2_base, int j, int hd) {
   return exp2(-2.0 * j / hd * log2_base) * 0.15915494309189533577;
 }
+// cos and sin of place * turns whole turns. The turns and then the quarters are taken off in 64 bits; what is left is at most an
+// eighth of a turn either way, where Taylor's series to the ninth and tenth power is within 2e-9 of sin and cos in 32 bits.
 __device__ __forceinline__ float2 cos_sin(double place, double turns) {
   double u = place * turns;
   u -= rint(u);
-  double s, c;
-  sincospi(2.0 * u, &s, &c);
-  return make_float2((float)c, (float)s);
+  const double q = rint(4.0 * u);
+  const float t = (float)(u - 0.25 * q);
+  const float a = __builtin_fmaf(t, 6.28318548f, t * -1.74845553e-7f);       // 2 pi in two parts
+  const float z = a * a;
+  const float s = __builtin_fmaf(a * z, __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, 2.75573192e-6f, -1.98412698e-4f), 8.33333333e-3f), -1.66666667e-1f), a);
+  const float c = __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, -2.75573192e-7f, 2.48015873e-5f), -1.38888889e-3f),
+                                                                     4.16666667e-2f), -0.5f), 1.0f);
+  const int k = (int)q;                          // -2 .. 2 quarters
+  const float x = k & 1 ? s : c, y = k & 1 ? c : s;
+  return make_float2(((k + 1) & 2) ? -x : x, (k & 2) ? -y : y);
 }
 __device__ __forceinline__ double place_of(const QkArgs &A, int64_t row) {
   return A.places ? (double)A.places[row] : (double)(row % A.T) + (double)A.pos;
 }
 
+// Sum over the LPH lanes of a head, in every one of them: within 16 lanes by exchanges of the vector unit, beyond through LDS.
+template <int CTRL> __device__ __forceinline__ float dpp_add(float v) {
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
 template <int LPH> __device__ __forceinline__ float head_sum(float v) {
-#pragma unroll
-  for (int o = LPH / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, WAVE);
+  v = dpp_add<0xB1>(v);                          // neighbours
+  v = dpp_add<0x4E>(v);                          // pairs
+  if (LPH >= 8) v = dpp_add<0x141>(v);           // halves of eight
+  if (LPH >= 16) v = dpp_add<0x140>(v);          // halves of sixteen
+  if (LPH >= 32) v += __shfl_xor(v, 16, WAVE);
+  if (LPH >= 64) v += __shfl_xor(v, 32, WAVE);
   return v;
 }
 __device__ __forceinline__ float sum4(v4f t) { return (t[0] + t[1]) + (t[2] + t[3]); }
+// 1 / sqrt(t): the hardware's and one Newton step
+__device__ __forceinline__ float inv_root(float t) {
+  const float y = __builtin_amdgcn_rsqf(t);
+  return __builtin_fmaf(0.5f * y, __builtin_fmaf(-t * y, y, 1.0f), y);
+}
 
-// A workgroup takes R rows at a time (R * hd/2 <= 256 angles, one per thread) and its 256 / LPH lane groups go through the
-// rows' heads, those of q and then those of k row by row.
+// What a workgroup keeps of its rows and the gains: [row][pair] cosines and sines, [side][hd].
+struct QkShared { float c[QK_ANGLES], s[QK_ANGLES], w[2][QK_VEC_HD]; };
+
+// A workgroup takes R rows at a time (R * hd/2 <= 256 angles, one per thread). Its wavefronts go through the rows' heads of q and
+// then of k, 64 / LPH heads at a time, so that all of a wavefront is on one side and what differs between the sides is scalar.
+struct QkPlan { int R, half, lq; unsigned mq, mk; };
+__device__ __forceinline__ void shared_gains(const QkArgs &A, QkShared &L) {
+  for (int i = threadIdx.x; i < 2 * A.hd; i += 256) L.w[i >= A.hd][i >= A.hd ? i - A.hd : i] = i >= A.hd ? A.s[1].w[i - A.hd] : A.s[0].w[i];
+}
+
+// A thread forms the angles of one pair, in every 256 / half-th row.
+__device__ __forceinline__ void shared_angles(const QkArgs &A, QkShared &L, int64_t row0, int nr, int half, double turns) {
+  const int step = 256 / half, r0 = threadIdx.x / half, j = threadIdx.x - r0 * half;
+  if (r0 >= step) return;
+  for (int r = r0; r < nr; r += step) {
+    const float2 cs = cos_sin(place_of(A, row0 + r), turns);
+    L.c[r * half + j] = cs.x;
+    L.s[r * half + j] = cs.y;
+  }
+}
+
 template <int LPH>
-__global__ __launch_bounds__(256) void qk_norm_rope_fwd_k(QkArgs A, int R) {
-  constexpr int G = 256 / LPH;
-  __shared__ float2 cs[256];
-  const int half = A.hd / 2, lq = A.hd / 8;
-  const int grp = threadIdx.x / LPH, li = min((int)threadIdx.x % LPH, lq - 1);
-  const bool live = (int)threadIdx.x % LPH < lq;
-  const int Hq = A.s[0].H, Ht = Hq + A.s[1].H;
+__global__ __launch_bounds__(256) void qk_norm_rope_fwd_k(QkArgs A, QkPlan P) {
+  constexpr int UPW = WAVE / LPH;                // heads that a wavefront takes at once
+  __shared__ QkShared L;
+  const int half = P.half, lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+  const int sub = lane / LPH, li = min(lane % LPH, P.lq - 1);
+  const bool mine = lane % LPH < P.lq;
   const float invd = 1.0f / (float)A.hd;
-  const int ar = threadIdx.x / half, aj = threadIdx.x % half;
-  const double turns = turns_per_place(A.log2_base, aj, A.hd);
-  v4f w[2][2];
-#pragma unroll
-  for (int s = 0; s < 2; s++)
-#pragma unroll
-    for (int p = 0; p < 2; p++) w[s][p] = reinterpret_cast<const v4f *>(A.s[s].w + p * half)[li];
-  for (int64_t row0 = (int64_t)blockIdx.x * R; row0 < A.rows; row0 += (int64_t)gridDim.x * R) {
-    const int nr = (int)min((int64_t)R, A.rows - row0);
-    __syncthreads();
-    if (ar < nr) cs[threadIdx.x] = cos_sin(place_of(A, row0 + ar), turns);
-    __syncthreads();
-    for (int u = grp; u < nr * Ht; u += G) {
-      const int rr = u / Ht, h = u - rr * Ht;
-      const bool isk = h >= Hq;
-      const QkSide &S = isk ? A.s[1] : A.s[0];
-      const int hh = isk ? h - Hq : h;
-      const float *x = S.x + (row0 + rr) * S.ldx + (int64_t)hh * A.hd;
-      v4f a = reinterpret_cast<const v4f *>(x)[li], b = reinterpret_cast<const v4f *>(x + half)[li];
-      const v4f q2 = a * a + b * b;
-      const float ss = head_sum<LPH>(live ? sum4(q2) : 0.f);
-      const float r = 1.0f / sqrtf(ss * invd + A.eps);
-      a = a * r * (isk ? w[1][0] : w[0][0]);
-      b = b * r * (isk ? w[1][1] : w[0][1]);
-      const v4f *cp = reinterpret_cast<const v4f *>(cs + rr * half + 4 * li);
-      const v4f c0 = cp[0], c1 = cp[1];
-      const v4f c = {c0[0], c0[2], c1[0], c1[2]}, sn = {c0[1], c0[3], c1[1], c1[3]};
-      float *o = S.o + (row0 + rr) * S.ldo + (int64_t)hh * A.hd;
-      if (live) {
-        reinterpret_cast<v4f *>(o)[li] = a * c - b * sn;
-        reinterpret_cast<v4f *>(o + half)[li] = a * sn + b * c;
-      }
+  const int64_t row0 = (int64_t)blockIdx.x * P.R;
+  const int nr = (int)min((int64_t)P.R, A.rows - row0);
+  const int nq = nr * A.s[0].H, nk = nr * A.s[1].H, nqw = (nq + UPW - 1) / UPW, nw = nqw + (nk + UPW - 1) / UPW;
+  shared_gains(A, L);
+  shared_angles(A, L, row0, nr, half, turns_per_place(A.log2_base, threadIdx.x % half, A.hd));
+  __syncthreads();
+  for (int i = wave; i < nw; i += 4) {
+    const int side = i >= nqw;
+    const QkSide &S = A.s[side];
+    const int u = (side ? i - nqw : i) * UPW + sub, n = side ? nk : nq;
+    const bool live = mine && u < n;
+    const int uc = min(u, n - 1);
+    const int rr = (int)__umulhi(2u * uc, side ? P.mk : P.mq), h = uc - rr * S.H;
+    const float *x = S.x + (row0 + rr) * S.ldx + (int64_t)h * A.hd;
+    v4f a = __builtin_nontemporal_load(reinterpret_cast<const v4f *>(x) + li), b = __builtin_nontemporal_load(reinterpret_cast<const v4f *>(x + half) + li);
+    const float ss = head_sum<LPH>(mine ? sum4(a * a + b * b) : 0.f);
+    const float r = inv_root(ss * invd + A.eps);
+    a = a * r * reinterpret_cast<const v4f *>(L.w[side])[li];
+    b = b * r * reinterpret_cast<const v4f *>(L.w[side] + half)[li];
+    const v4f c = reinterpret_cast<const v4f *>(L.c + rr * half)[li], sn = reinterpret_cast<const v4f *>(L.s + rr * half)[li];
+    float *o = S.o + (row0 + rr) * S.ldo + (int64_t)h * A.hd;
+    if (live) {
+      __builtin_nontemporal_store(a * c - b * sn, reinterpret_cast<v4f *>(o) + li);
+      __builtin_nontemporal_store(a * sn + b * c, reinterpret_cast<v4f *>(o + half) + li);
     }
   }
 }
 
 template <int LPH>
-__global__ __launch_bounds__(256) void qk_norm_rope_bwd_k(QkArgs A, int R) {
-  constexpr int G = 256 / LPH;
-  __shared__ float2 cs[256];
-  __shared__ v4f red[2][256];                    // [half][lane group][lane]: the gain sums of one side
-  const int half = A.hd / 2, lq = A.hd / 8;
-  const int grp = threadIdx.x / LPH, li = min((int)threadIdx.x % LPH, lq - 1);
-  const bool live = (int)threadIdx.x % LPH < lq;
-  const int Hq = A.s[0].H, Ht = Hq + A.s[1].H;
+__global__ __launch_bounds__(256) void qk_norm_rope_bwd_k(QkArgs A, QkPlan P) {
+  constexpr int UPW = WAVE / LPH;
+  __shared__ QkShared L;
+  __shared__ v4f red[2][4][QK_VEC_HD / 4];       // [side][wavefront][column]: the gain sums
+  const int half = P.half, lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+  const int sub = lane / LPH, li = min(lane % LPH, P.lq - 1);
+  const bool mine = lane % LPH < P.lq;
   const float invd = 1.0f / (float)A.hd;
   const bool turn = A.s[0].rot | A.s[1].rot;
-  const int ar = threadIdx.x / half, aj = threadIdx.x % half;
-  const double turns = turn ? turns_per_place(A.log2_base, aj, A.hd) : 0.0;
-  v4f w[2][2], dw[2][2];
+  const double turns = turn ? turns_per_place(A.log2_base, threadIdx.x % half, A.hd) : 0.0;
+  v4f dw[2][2];
 #pragma unroll
-  for (int s = 0; s < 2; s++)
-#pragma unroll
-    for (int p = 0; p < 2; p++) {
-      w[s][p] = reinterpret_cast<const v4f *>(A.s[s].w + p * half)[li];
-      dw[s][p] = v4f{0, 0, 0, 0};
-    }
-  for (int64_t row0 = (int64_t)blockIdx.x * R; row0 < A.rows; row0 += (int64_t)gridDim.x * R) {
-    const int nr = (int)min((int64_t)R, A.rows - row0);
+  for (int s = 0; s < 2; s++) dw[s][0] = dw[s][1] = v4f{0, 0, 0, 0};
+  shared_gains(A, L);
+  __syncthreads();
+  for (int64_t row0 = (int64_t)blockIdx.x * P.R; row0 < A.rows; row0 += (int64_t)gridDim.x * P.R) {
+    const int nr = (int)min((int64_t)P.R, A.rows - row0);
+    const int nq = nr * A.s[0].H, nk = nr * A.s[1].H, nqw = (nq + UPW - 1) / UPW, nw = nqw + (nk + UPW - 1) / UPW;
     if (turn) {
       __syncthreads();
-      if (ar < nr) cs[threadIdx.x] = cos_sin(place_of(A, row0 + ar), turns);
+      shared_angles(A, L, row0, nr, half, turns);
       __syncthreads();
     }
-    for (int u = grp; u < nr * Ht; u += G) {
-      const int rr = u / Ht, h = u - rr * Ht;
-      const bool isk = h >= Hq;
-      const QkSide &S = isk ? A.s[1] : A.s[0];
-      const int hh = isk ? h - Hq : h;
-      const int64_t xo = (row0 + rr) * S.ldx + (int64_t)hh * A.hd, go = (row0 + rr) * S.ldo + (int64_t)hh * A.hd;
-      const v4f a = reinterpret_cast<const v4f *>(S.x + xo)[li], b = reinterpret_cast<const v4f *>(S.x + xo + half)[li];
-      v4f ga = reinterpret_cast<const v4f *>(S.g + go)[li], gb = reinterpret_cast<const v4f *>(S.g + go + half)[li];
+    for (int i = wave; i < nw; i += 4) {
+      const int side = i >= nqw;
+      const QkSide &S = A.s[side];
+      const int u = (side ? i - nqw : i) * UPW + sub, n = side ? nk : nq;
+      const bool live = mine && u < n;
+      const int uc = min(u, n - 1);
+      const int rr = (int)__umulhi(2u * uc, side ? P.mk : P.mq), h = uc - rr * S.H;
+      const int64_t xo = (row0 + rr) * S.ldx + (int64_t)h * A.hd, go = (row0 + rr) * S.ldo + (int64_t)h * A.hd;
+      const v4f a = __builtin_nontemporal_load(reinterpret_cast<const v4f *>(S.x + xo) + li);
+      const v4f b = __builtin_nontemporal_load(reinterpret_cast<const v4f *>(S.x + xo + half) + li);
+      v4f ga = __builtin_nontemporal_load(reinterpret_cast<const v4f *>(S.g + go) + li);
+      v4f gb = __builtin_nontemporal_load(reinterpret_cast<const v4f *>(S.g + go + half) + li);
       v4f oa = {0, 0, 0, 0}, ob = {0, 0, 0, 0};
       if (S.old) {
-        oa = reinterpret_cast<const v4f *>(S.old + xo)[li];
-        ob = reinterpret_cast<const v4f *>(S.old + xo + half)[li];
+        oa = __builtin_nontemporal_load(reinterpret_cast<const v4f *>(S.old + xo) + li);
+        ob = __builtin_nontemporal_load(reinterpret_cast<const v4f *>(S.old + xo + half) + li);
       }
       if (S.rot) {
-        const v4f *cp = reinterpret_cast<const v4f *>(cs + rr * half + 4 * li);
-        const v4f c0 = cp[0], c1 = cp[1];
-        const v4f c = {c0[0], c0[2], c1[0], c1[2]}, sn = {c0[1], c0[3], c1[1], c1[3]};
+        const v4f c = reinterpret_cast<const v4f *>(L.c + rr * half)[li], sn = reinterpret_cast<const v4f *>(L.s + rr * half)[li];
         const v4f ta = ga * c + gb * sn;
         gb = gb * c - ga * sn;
         ga = ta;
       }
-      const v4f wa = isk ? w[1][0] : w[0][0], wb = isk ? w[1][1] : w[0][1];
-      const float ss = head_sum<LPH>(live ? sum4(a * a + b * b) : 0.f);
-      const float dot = head_sum<LPH>(live ? sum4(ga * wa * a + gb * wb * b) : 0.f);
-      const float r = 1.0f / sqrtf(ss * invd + A.eps);
+      const v4f wa = reinterpret_cast<const v4f *>(L.w[side])[li], wb = reinterpret_cast<const v4f *>(L.w[side] + half)[li];
+      const float ss = head_sum<LPH>(mine ? sum4(a * a + b * b) : 0.f);
+      const float dot = head_sum<LPH>(mine ? sum4(ga * wa * a + gb * wb * b) : 0.f);
+      const float r = inv_root(ss * invd + A.eps);
       const float k2 = r * r * r * dot * invd;
       if (S.o && live) {
-        reinterpret_cast<v4f *>(S.o + xo)[li] = wa * ga * r - a * k2 + oa;
-        reinterpret_cast<v4f *>(S.o + xo + half)[li] = wb * gb * r - b * k2 + ob;
+        __builtin_nontemporal_store(wa * ga * r - a * k2 + oa, reinterpret_cast<v4f *>(S.o + xo) + li);
+        __builtin_nontemporal_store(wb * gb * r - b * k2 + ob, reinterpret_cast<v4f *>(S.o + xo + half) + li);
       }
-      const v4f ta = ga * a * r, tb = gb * b * r;
-      if (isk) { dw[1][0] += ta; dw[1][1] += tb; }
+      const float rl = u < n ? r : 0.f;          // a head past the last one adds nothing
+      const v4f ta = u < n ? ga * a * rl : v4f{0, 0, 0, 0}, tb = u < n ? gb * b * rl : v4f{0, 0, 0, 0};
+      if (side) { dw[1][0] += ta; dw[1][1] += tb; }
       else { dw[0][0] += ta; dw[0][1] += tb; }
     }
   }
-  // the lane groups' sums in group order, one partial row per workgroup and side
+  // the sums of a wavefront's heads by exchanges, then the four wavefronts' in order: one partial row per workgroup and side
 #pragma unroll
-  for (int s = 0; s < 2; s++) {
-    if (!A.s[s].part) continue;
-    __syncthreads();
-    red[0][threadIdx.x] = dw[s][0];
-    red[1][threadIdx.x] = dw[s][1];
-    __syncthreads();
-    const int t = threadIdx.x;
-    if (t < 2 * lq) {
-      const int p = t / lq, l = t - p * lq;
-      v4f sum = red[p][l];
-      for (int q = 1; q < G; q++) sum += red[p][q * LPH + l];
-      reinterpret_cast<v4f *>(A.s[s].part + (size_t)blockIdx.x * A.hd + p * half)[l] = sum;
+  for (int s = 0; s < 2; s++)
+#pragma unroll
+    for (int p = 0; p < 2; p++) {
+#pragma unroll
+      for (int o = LPH; o < WAVE; o *= 2)
+#pragma unroll
+        for (int j = 0; j < 4; j++) dw[s][p][j] += __shfl_xor(dw[s][p][j], o, WAVE);
+      if (sub == 0 && mine) red[s][wave][p * P.lq + li] = dw[s][p];
     }
+  __syncthreads();
+  for (int t = threadIdx.x; t < 4 * P.lq; t += 256) {
+    const int s = t >= 2 * P.lq, c = t - s * 2 * P.lq;
+    if (A.s[s].part)
+      reinterpret_cast<v4f *>(A.s[s].part + (size_t)blockIdx.x * A.hd)[c] = ((red[s][0][c] + red[s][1][c]) + red[s][2][c]) + red[s][3][c];
   }
 }
 
@@ -281,16 +323,30 @@ static bool qk_vec(int hd, const QkSide &q, const QkSide &k) {
   }
   return bits % 16 == 0;
 }
-static int qk_rows_at_once(int hd) { return std::max(1, 256 / (hd / 2)); }
-// workgroups of a backward call, vector or generic kernel alike: one partial row of gain sums each
-static int qk_bwd_groups(gt_ctx *ctx, int64_t rows, int hd) {
-  const int R = hd % 8 == 0 && hd <= QK_VEC_HD ? qk_rows_at_once(hd) : 1;
-  return (int)std::min<int64_t>(cdiv(rows, R), (int64_t)ctx->num_cu * 4);
+#define QK_LPH_OF(hd) ((hd) <= 32 ? 4 : (hd) <= 64 ? 8 : (hd) <= 128 ? 16 : (hd) <= 256 ? 32 : 64)
+// Rows to a workgroup such that its wavefronts have `passes` heads (or groups of heads) to go through in all, as far as LDS holds
+// their angles.
+static int qk_rows_at_once(int heads, int hd, int passes) {
+  return (int)std::max<int64_t>(1, std::min<int64_t>(QK_ANGLES / (hd / 2), cdiv((int64_t)passes * (WAVE / QK_LPH_OF(hd)), heads)));
+}
+static QkPlan qk_plan(int hd, int R, int Hq, int Hk) {
+  // heads are fewer than 2^15 per group of rows, so that u / H is the high word of 2 u * ceil(2^31 / H)
+  return {R, hd / 2, hd / 8, (unsigned)((0x80000000ull + Hq - 1) / Hq), (unsigned)((0x80000000ull + Hk - 1) / Hk)};
+}
+// A backward call's workgroups, one partial row of gain sums each, of the vector and of the generic kernel alike; and the rows that
+// each takes at a time, fewer where that lets every workgroup have the same number of turns.
+static int qk_bwd_rows(gt_ctx *ctx, int64_t rows, int heads, int hd) {
+  if (hd % 8 || hd > QK_VEC_HD) return 1;
+  const int64_t groups = (int64_t)ctx->num_cu * QK_BWD_PER_CU, turns = cdiv(rows, groups * qk_rows_at_once(heads, hd, QK_BWD_PASSES));
+  return (int)cdiv(rows, groups * turns);
+}
+static int qk_bwd_groups(gt_ctx *ctx, int64_t rows, int heads, int hd) {
+  return (int)std::min<int64_t>(cdiv(rows, qk_bwd_rows(ctx, rows, heads, hd)), (int64_t)ctx->num_cu * QK_BWD_PER_CU);
 }
 
 #define QK_LPH(hd, CALL) do { \
-    if ((hd) <= 32) { CALL(4); } else if ((hd) <= 64) { CALL(8); } else if ((hd) <= 128) { CALL(16); } \
-    else if ((hd) <= 256) { CALL(32); } else { CALL(64); } } while (0)
+    switch (QK_LPH_OF(hd)) { case 4: CALL(4); break; case 8: CALL(8); break; case 16: CALL(16); break; case 32: CALL(32); break; \
+      default: CALL(64); } } while (0)
 
 static int qk_check(gt_ctx *ctx, const char *who, int rows, int T, int Hq, int Hkv, int hd, double base, gt_buf places, gt_buf q, int64_t ldq,
                     gt_buf wq, gt_buf k, int64_t ldk, gt_buf wk, int64_t ldqo, int64_t ldko) {
@@ -317,10 +373,10 @@ static int qk_bwd(gt_ctx *ctx, const char *who, int rows, int T, int Hq, int Hkv
   A.places = P<const int>(places);
   A.log2_base = log2(base);
   A.rows = rows; A.T = T; A.pos = pos; A.hd = hd; A.eps = eps;
-  const int nb = qk_bwd_groups(ctx, rows, hd);
+  const int nb = qk_bwd_groups(ctx, rows, Hq + Hkv, hd);
   if (qk_vec(hd, A.s[0], A.s[1])) {
-    const int R = qk_rows_at_once(hd);
-#define CALL(L) hipLaunchKernelGGL((qk_norm_rope_bwd_k<L>), dim3((unsigned)nb), dim3(256), 0, ctx->stream, A, R)
+    const QkPlan plan = qk_plan(hd, qk_bwd_rows(ctx, rows, Hq + Hkv, hd), Hq, Hkv);
+#define CALL(L) hipLaunchKernelGGL((qk_norm_rope_bwd_k<L>), dim3((unsigned)nb), dim3(256), 0, ctx->stream, A, plan)
     QK_LPH(hd, CALL);
 #undef CALL
   } else {
@@ -347,9 +403,9 @@ int gt_qk_norm_rope_fwd(gt_ctx *ctx, int rows, int T, int Hq, int Hkv, int hd, f
   A.log2_base = log2(base);
   A.rows = rows; A.T = T; A.pos = pos; A.hd = hd; A.eps = eps;
   if (qk_vec(hd, A.s[0], A.s[1])) {
-    const int R = qk_rows_at_once(hd);
-    const unsigned nb = (unsigned)std::min<int64_t>(cdiv(rows, R), (int64_t)ctx->num_cu * 8);
-#define CALL(L) hipLaunchKernelGGL((qk_norm_rope_fwd_k<L>), dim3(nb), dim3(256), 0, ctx->stream, A, R)
+    const QkPlan plan = qk_plan(hd, (int)std::min<int64_t>(qk_rows_at_once(Hq + Hkv, hd, QK_FWD_PASSES), std::max(1, rows / ctx->num_cu)), Hq, Hkv);
+    const unsigned nb = (unsigned)cdiv(rows, plan.R);
+#define CALL(L) hipLaunchKernelGGL((qk_norm_rope_fwd_k<L>), dim3(nb), dim3(256), 0, ctx->stream, A, plan)
     QK_LPH(hd, CALL);
 #undef CALL
   } else {
@@ -375,7 +431,7 @@ int gt_qk_norm_rope_bwd(gt_ctx *ctx, int rows, int T, int Hq, int Hkv, int hd, f
     return 0;
   }
   if (!dq && !dk && !dwq && !dwk) return 0;
-  const int nb = qk_bwd_groups(ctx, rows, hd);
+  const int nb = qk_bwd_groups(ctx, rows, Hq + Hkv, hd);
   const size_t one = ((size_t)nb * hd + 3) / 4 * 4;
   float *parts = nullptr;
   if (dwq || dwk) {
@@ -396,9 +452,9 @@ int gt_qk_norm_rope_bwd(gt_ctx *ctx, int rows, int T, int Hq, int Hkv, int hd, f
   return gt_colsum_group(ctx, n, sp, sn, sw, sd, sa);
 }
 
-int gt_qk_norm_rope_parts_rows(gt_ctx *ctx, int rows, int hd, int *nparts) {
+int gt_qk_norm_rope_parts_rows(gt_ctx *ctx, int rows, int Hq, int Hkv, int hd, int *nparts) {
   if (!ctx || !nparts) return 1;
-  *nparts = rows >= 1 && hd >= 2 && hd % 2 == 0 && hd <= QK_MAX_HD ? qk_bwd_groups(ctx, rows, hd) : 0;
+  *nparts = rows >= 1 && Hq >= 1 && Hkv >= 1 && hd >= 2 && hd % 2 == 0 && hd <= QK_MAX_HD ? qk_bwd_groups(ctx, rows, Hq + Hkv, hd) : 0;
   return 0;
 }
 

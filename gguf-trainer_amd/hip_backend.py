@@ -1301,7 +1301,7 @@ class HipBackend:
             dwk, awk = self._gdst(kw) if wants_k else (0, 0)
             nparts = C.c_int(0)
             if self.defer_norm_dw and (dwq or dwk):
-                check(self._ctx, lib.gt_qk_norm_rope_parts_rows(self._ctx, rows, hd, C.byref(nparts)), "qkNormRope.bwd")
+                check(self._ctx, lib.gt_qk_norm_rope_parts_rows(self._ctx, rows, Hq, Hkv, hd, C.byref(nparts)), "qkNormRope.bwd")
             if nparts.value > 0:
                 pq, pk = (self._scratch_buf(nparts.value * hd * 4) if d else 0 for d in (dwq, dwk))
                 check(self._ctx, lib.gt_qk_norm_rope_bwd_parts(self._ctx, rows, T, Hq, Hkv, hd, eps, base, pos_offset, places, qd, ldq, qwd, gq, ldq,

@@ -77,7 +77,7 @@ _SIG = {
     "gt_qk_norm_rope_fwd": [ctxp, i32, i32, i32, i32, i32, f32, f64, i32, buf, buf, i64, buf, buf, i64, buf, i64, buf, buf, i64],
     "gt_qk_norm_rope_bwd": [ctxp, i32, i32, i32, i32, i32, f32, f64, i32, buf, buf, i64, buf, buf, i64, i32, buf, i32, buf, i32,
                             buf, i64, buf, buf, i64, i32, buf, i32, buf, i32],
-    "gt_qk_norm_rope_parts_rows": [ctxp, i32, i32, C.POINTER(i32)],
+    "gt_qk_norm_rope_parts_rows": [ctxp, i32, i32, i32, i32, C.POINTER(i32)],
     "gt_qk_norm_rope_bwd_parts": [ctxp, i32, i32, i32, i32, i32, f32, f64, i32, buf, buf, i64, buf, buf, i64, i32, buf, i32, buf,
                                   buf, i64, buf, buf, i64, i32, buf, i32, buf],
     "gt_attn_fwd": [ctxp, i32, i32, i32, i32, i32, i32, buf, buf, buf, buf, buf],

@@ -81,7 +81,7 @@ const SYMBOLS = {
   gt_rope:               { parameters: [ptr, i32, i32, i32, i32, f64, i32, i32, u64, u64, i32], result: i32 },
   gt_qk_norm_rope_fwd:   { parameters: [ptr, i32, i32, i32, i32, i32, f32, f64, i32, u64, u64, i64, u64, u64, i64, u64, i64, u64, u64, i64], result: i32 },
   gt_qk_norm_rope_bwd:   { parameters: [ptr, i32, i32, i32, i32, i32, f32, f64, i32, u64, u64, i64, u64, u64, i64, i32, u64, i32, u64, i32, u64, i64, u64, u64, i64, i32, u64, i32, u64, i32], result: i32 },
-  gt_qk_norm_rope_parts_rows: { parameters: [ptr, i32, i32, buf], result: i32 },
+  gt_qk_norm_rope_parts_rows: { parameters: [ptr, i32, i32, i32, i32, buf], result: i32 },
   gt_qk_norm_rope_bwd_parts: { parameters: [ptr, i32, i32, i32, i32, i32, f32, f64, i32, u64, u64, i64, u64, u64, i64, i32, u64, i32, u64, u64, i64, u64, u64, i64, i32, u64, i32, u64], result: i32 },
   gt_rope_pair:          { parameters: [ptr, i32, i32, i32, f64, i32, i32, i32, u64, u64, i32, i32, u64, u64, i32], result: i32 },
   gt_attn_fwd:           { parameters: [ptr, i32, i32, i32, i32, i32, i32, u64, u64, u64, u64, u64], result: i32 },

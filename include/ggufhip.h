@@ -252,7 +252,7 @@ int gt_qk_norm_rope_fwd(gt_ctx *ctx, int rows, int T, int Hq, int Hkv, int hd, f
 int gt_qk_norm_rope_bwd(gt_ctx *ctx, int rows, int T, int Hq, int Hkv, int hd, float eps, double base, int pos, gt_buf places,
                         gt_buf q, int64_t ldq, gt_buf wq, gt_buf gq, int64_t ldgq, int rot_q, gt_buf dq, int acc_q, gt_buf dwq, int acc_wq,
                         gt_buf k, int64_t ldk, gt_buf wk, gt_buf gk, int64_t ldgk, int rot_k, gt_buf dk, int acc_k, gt_buf dwk, int acc_wk);
-int gt_qk_norm_rope_parts_rows(gt_ctx *ctx, int rows, int hd, int *nparts);
+int gt_qk_norm_rope_parts_rows(gt_ctx *ctx, int rows, int Hq, int Hkv, int hd, int *nparts);
 int gt_qk_norm_rope_bwd_parts(gt_ctx *ctx, int rows, int T, int Hq, int Hkv, int hd, float eps, double base, int pos, gt_buf places,
                               gt_buf q, int64_t ldq, gt_buf wq, gt_buf gq, int64_t ldgq, int rot_q, gt_buf dq, int acc_q, gt_buf parts_q,
                               gt_buf k, int64_t ldk, gt_buf wk, gt_buf gk, int64_t ldgk, int rot_k, gt_buf dk, int acc_k, gt_buf parts_k);

@@ -352,7 +352,7 @@ def test_partial_rows_and_column_sums_give_the_same_bits(gpu, bufs, hd):
     L = mod("lib")
     q, k, wq, wk, gq, gk = inputs(rows, Hq, Hkv, hd, 15)
     n = C.c_int(0)
-    L.check(gpu.ctx, L.lib.gt_qk_norm_rope_parts_rows(gpu.ctx, rows, hd, C.byref(n)), "rows")
+    L.check(gpu.ctx, L.lib.gt_qk_norm_rope_parts_rows(gpu.ctx, rows, Hq, Hkv, hd, C.byref(n)), "rows")
     assert n.value >= 1
     pq, pk = bufs.raw(n.value * hd * 4), bufs.raw(n.value * hd * 4)
     dq, dk, dwq, dwk = bufs.raw(q.nbytes), bufs.raw(k.nbytes), bufs.raw(hd * 4), bufs.raw(hd * 4)
@@ -432,7 +432,7 @@ def test_refusals(gpu, bufs):
             parts(*a)
     with pytest.raises(L.HipError, match="rows 0"):
         parts(b, b, rows=0)
-    assert L.lib.gt_qk_norm_rope_parts_rows(gpu.ctx, 4, 8, None) != 0
+    assert L.lib.gt_qk_norm_rope_parts_rows(gpu.ctx, 4, 2, 1, 8, None) != 0
     gpu.sync([])                                     # nothing above was launched: the stream is fine
 
 
