@@ -373,6 +373,7 @@ def run_workload(mods, config, steps, warmup, a, headline):
     gpu.fuse_sibling_dx = "sibling_dx" not in a.no_fuse
     gpu.fuse_residual_add = "residual_add" not in a.no_fuse
     gpu.alias_add_grads = "add_grads" not in a.no_fuse
+    gpu.fuse_qk_norm_rope = a.fuse_qk_norm_rope
     for kv in a.set:
         key, _, val = kv.partition("=")
         gpu.set_option(key, int(val))
@@ -385,12 +386,12 @@ def run_workload(mods, config, steps, warmup, a, headline):
                 outd, ind = arch.layer_shapes(cfg)[k]
                 adapters[f"L{l}.{k}"] = ((0.02 * rs.standard_normal((rank, ind))).astype(np.float32), np.zeros((outd, rank), np.float32))
         trainable = arch.apply_lora(model, rank, 16.0, adapters)
-        opt = optim.AdamWHip(gpu, trainable, lr=1e-3, beta1=0.9, beta2=0.95, weight_decay=0.0, clip=1.0)
+        opt = optim.AdamWHip(gpu, trainable, lr=1e-3, beta1=0.9, beta2=0.95, weight_decay=0.0, clip=1.0, state_bits=a.adamw_bits)
     elif wl.get("muon"):
         mu, aux = model.param_groups()
-        opt = optim.MuonHip(gpu, mu, aux, lr=0.01, momentum=0.95, nesterov=True, ns_steps=5, aux={"lr": 3e-3})
+        opt = optim.MuonHip(gpu, mu, aux, lr=0.01, momentum=0.95, nesterov=True, ns_steps=5, aux={"lr": 3e-3, "state_bits": a.adamw_bits})
     else:
-        opt = optim.AdamWHip(gpu, model.params(), lr=1e-3, beta1=0.9, beta2=0.95, weight_decay=0.1, clip=1.0)
+        opt = optim.AdamWHip(gpu, model.params(), lr=1e-3, beta1=0.9, beta2=0.95, weight_decay=0.1, clip=1.0, state_bits=a.adamw_bits)
     ag.set_checkpointing(bool(wl.get("recompute")))
     total = steps + warmup
     if config == 3:
@@ -454,7 +455,7 @@ def run_workload(mods, config, steps, warmup, a, headline):
         gpu.start_profile("muon" if wl.get("muon") else "adamw")
         step(total - 1)
         op = gpu.stop_profile()
-        res["opt_prof"] = op.get("adamw")
+        res["opt_prof"] = op.get("adamw8" if a.adamw_bits == 8 else "adamw")
         res["opt_sustained"] = None
         if headline and not wl.get("muon") and not wl.get("lora"):
             # ten AdamW steps back to back inside one event pair (gradients as the last backward left them): the kernel's rate
@@ -463,11 +464,17 @@ def run_workload(mods, config, steps, warmup, a, headline):
             Lm = importlib.import_module(f"{PKG}.lib")
             gpu.ensure_grads_defined(opt.params)
             ms = C.c_double()
-            for _ in range(2):
-                Lm.check(gpu.ctx, Lm.lib.gt_adamw_step(gpu.ctx, opt._h, 0.0, 0.5, 0.5), "gt_adamw_step")      # lr 0: the weights stay put
+
+            def still(k):                        # lr 0: the weights stay put
+                if a.adamw_bits == 8:
+                    Lm.check(gpu.ctx, Lm.lib.gt_adamw8_step(gpu.ctx, opt._h, 0.0, 0.5, 0.5, k), "gt_adamw8_step")
+                else:
+                    Lm.check(gpu.ctx, Lm.lib.gt_adamw_step(gpu.ctx, opt._h, 0.0, 0.5, 0.5), "gt_adamw_step")
+            for k in range(2):
+                still(k)
             Lm.check(gpu.ctx, Lm.lib.gt_timer_start(gpu.ctx), "gt_timer_start")
-            for _ in range(10):
-                Lm.check(gpu.ctx, Lm.lib.gt_adamw_step(gpu.ctx, opt._h, 0.0, 0.5, 0.5), "gt_adamw_step")
+            for k in range(10):
+                still(k)
             Lm.check(gpu.ctx, Lm.lib.gt_timer_stop(gpu.ctx, C.byref(ms)), "gt_timer_stop")
             res["opt_sustained"] = ms.value / 10
         if wl.get("muon") and op.get("muon"):
@@ -625,6 +632,9 @@ def main():
                     help="attention recomputes Q.K^T in the backward instead of keeping the forward's scores (saves B*Hq*T*T*4 bytes per layer)")
     ap.add_argument("--no-fuse", action="append", default=[], choices=["sibling_dx", "residual_add", "add_grads"],
                     help="switch one of the host-side launch fusions off for an A/B run (repeatable)")
+    ap.add_argument("--fuse-qk-norm-rope", action="store_true",
+                    help="models with QK-norm: the norms and rotations of q and k as one op (HipBackend.fuse_qk_norm_rope)")
+    ap.add_argument("--adamw-bits", type=int, default=32, choices=(8, 32), help="how AdamW's moments are held")
     ap.add_argument("--set", action="append", default=[], metavar="KEY=VALUE",
                     help="library option for an A/B run, e.g. attn.keep_ds=0 (dQ recomputes the scores) or gemm.staged=1")
     ap.add_argument("--profile-all", action="store_true",
@@ -650,7 +660,7 @@ def main():
     if kernels is not None and r["opt_prof"] and a.config == 3:
         ms, cnt, work = r["opt_prof"]
         kernels[f"AdamW step, {r['n_params']} params, clip on"] = {
-            "kernel": "adamw", "bound": "hbm", "us_per_launch": round(1e3 * ms / cnt, 1),
+            "kernel": "adamw8" if a.adamw_bits == 8 else "adamw", "bound": "hbm", "us_per_launch": round(1e3 * ms / cnt, 1),
             "achieved": round(work / (ms * 1e-3) / 1e12, 3), "unit": "TB/s", "frac": round(work / (ms * 1e-3) / PEAK_HBM, 4),
             "launch": "the one step after a training step (three launches: sum of squares, clip scale, update)"}
         if r.get("opt_sustained"):
