@@ -22,6 +22,8 @@
 // largest moments are one exchange within the wavefront and no LDS is used. About 60 vector operations per element: at
 // twice that (library roots and divisions, float comparisons for the block's largest) they were as long as the memory's time.
 #include <algorithm>
+#include <exception>
+#include <utility>
 #include "optim.h"
 
 typedef float v4f __attribute__((ext_vector_type(4)));
@@ -31,6 +33,7 @@ typedef float v2f __attribute__((ext_vector_type(2)));
 #define CHUNK8 1024                              // four blocks, one to a wavefront
 #define NORM8_PER_CU 8                           // workgroups of the norm's kernel
 #define NORM8_GROUPS 2048
+#define SLICE8_CHUNKS (1 << 22)                  // chunks to a launch: a grid's threads are counted in 32 bits
 #define FOLD8_CHUNKS 2048                        // up to here the update's workgroups add up the norm's sums themselves
 // The chunk table's pointers come out of memory, where the compiler cannot see that they are global: without this its loads
 // take the flat path, which also waits for LDS.
@@ -121,10 +124,10 @@ __device__ __forceinline__ void encode_block(const float (&m)[4], const float (&
   // magnitudes order as their bits do
   unsigned am[4], av[4];
 #pragma unroll
-  for (int j = 0; j < 4; j++) { am[j] = __float_as_uint(m[j]) & 0x7fffffffu; av[j] = __float_as_uint(v[j]) & 0x7fffffffu; }
+  for (int j = 0; j < 4; j++) { am[j] = __float_as_uint(m[j]) & 0x7fffffffu; av[j] = __float_as_uint(v[j]); }
   unsigned tm = wave_umax(max(max(am[0], am[1]), max(am[2], am[3])));
   unsigned tv = wave_umax(max(max(av[0], av[1]), max(av[2], av[3])));
-  if (max(tm, tv) >= FINITE_BITS) {              // an infinity or a NaN: the exponents go by what is finite
+  if (max(tm, tv) >= FINITE_BITS) {              // an infinity, a NaN, a second moment below zero: the exponents go by the others
     tm = tv = 0;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -304,7 +307,7 @@ __global__ __launch_bounds__(256) void state8_write_k(int64_t size, unsigned cha
     float mm[4] = {0, 0, 0, 0}, vv[4] = {0, 0, 0, 0}, rr[4];
     const unsigned half[4] = {0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
 #pragma unroll
-    for (int j = 0; j < 4; j++) if (i0 + j < n) { mm[j] = m[b * BLK8 + i0 + j]; vv[j] = v[b * BLK8 + i0 + j]; }
+    for (int j = 0; j < 4; j++) if (i0 + j < n) { mm[j] = m[b * BLK8 + i0 + j]; vv[j] = v[b * BLK8 + i0 + j] + 0.f; }      // -0 becomes 0
 #pragma unroll
     for (int j = 0; j < 4; j++) rr[j] = root(vv[j]);
     unsigned mc, rc;
@@ -324,17 +327,40 @@ int gt_adamw8_create(gt_ctx *ctx, int n, const gt_buf *w, const gt_buf *g, const
   GT_REQUIRE(ctx, n >= 0 && out && (n == 0 || (w && g && m && r && e && sizes)), "gt_adamw8_create: bad arguments");
   int64_t blocks = 0, chunks = 0;
   for (int i = 0; i < n; i++) {
-    GT_REQUIRE(ctx, w[i] && g[i] && m[i] && r[i] && e[i] && sizes[i] >= 0, "gt_adamw8_create: tensor %d has a null buffer or a negative size", i);
+    GT_REQUIRE(ctx, w[i] && g[i] && m[i] && r[i] && e[i] && sizes[i] >= 0 && sizes[i] <= (int64_t)1 << 40,
+               "gt_adamw8_create: tensor %d has a null buffer or a size that is negative or more than 2^40", i);
     GT_REQUIRE(ctx, (w[i] | g[i]) % 4 == 0 && e[i] % 2 == 0, "gt_adamw8_create: tensor %d: a buffer is not aligned to its elements", i);
     blocks += cdiv(sizes[i], BLK8);
     chunks += cdiv(sizes[i], CHUNK8);
   }
   GT_REQUIRE(ctx, blocks <= 0xffffffffll && chunks <= 0x7fffffffll, "gt_adamw8_create: %lld blocks are more than a group can number", (long long)blocks);
-  gt_adamw *o = new gt_adamw();
+  // two tensors that share what a step writes would be stepped by two workgroups at once
+  std::vector<std::pair<uint64_t, uint64_t>> spans;
+  std::vector<Chunk8> ch;
+  gt_adamw *o = nullptr;
+  try {
+    spans.reserve((size_t)n * 4);
+    ch.reserve((size_t)chunks);
+    o = new gt_adamw();
+    o->tensors8.reserve((size_t)n);
+  } catch (const std::exception &) {
+    delete o;
+    GT_FAIL(ctx, "gt_adamw8_create: no host memory for a table of %lld chunks", (long long)chunks);
+  }
+  for (int i = 0; i < n; i++)
+    if (sizes[i]) {
+      const uint64_t s = (uint64_t)sizes[i];
+      for (auto p : {std::make_pair(w[i], s * 4), std::make_pair(m[i], s), std::make_pair(r[i], s), std::make_pair(e[i], (uint64_t)cdiv(sizes[i], BLK8) * 2)})
+        spans.push_back({p.first, p.first + p.second});
+    }
+  std::sort(spans.begin(), spans.end());
+  for (size_t i = 1; i < spans.size(); i++)
+    if (spans[i].first < spans[i - 1].second) {
+      delete o;
+      GT_FAIL(ctx, "gt_adamw8_create: two of the buffers that a step writes overlap (a tensor listed twice?)");
+    }
   o->bits8 = true;
   o->n = n; o->beta1 = beta1; o->beta2 = beta2; o->eps = eps; o->wd = weight_decay; o->clip = clip;
-  std::vector<Chunk8> ch;
-  ch.reserve((size_t)chunks);
   unsigned block = 0;
   for (int i = 0; i < n; i++) {
     o->tensors8.push_back({P<unsigned char>(m[i]), P<unsigned char>(r[i]), P<signed char>(e[i]), sizes[i]});
@@ -384,8 +410,11 @@ int gt_adamw8_step(gt_ctx *ctx, gt_adamw *o, double lr, double bc1, double bc2, 
     hipLaunchKernelGGL(adamw8_scale_k, dim3(1), dim3(256), 0, ctx->stream, o->sums8, nsums, o->clip, o->scale);
     GT_LAUNCHED(ctx);
   }
-  hipLaunchKernelGGL(adamw8_update_k, dim3((unsigned)o->nchunks), dim3(256), 0, ctx->stream, o->chunks8, o->sums8, fold ? nsums : 0, o->clip, o->scale, h);
-  GT_LAUNCHED(ctx);
+  for (int k = 0; k < o->nchunks; k += SLICE8_CHUNKS) {
+    const unsigned nb = (unsigned)std::min(SLICE8_CHUNKS, o->nchunks - k);
+    hipLaunchKernelGGL(adamw8_update_k, dim3(nb), dim3(256), 0, ctx->stream, o->chunks8 + k, o->sums8, fold ? nsums : 0, o->clip, o->scale, h);
+    GT_LAUNCHED(ctx);
+  }
   return 0;
 }
 

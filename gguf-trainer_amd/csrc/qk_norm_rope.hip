@@ -30,6 +30,7 @@ typedef float v4f __attribute__((ext_vector_type(4)));
 #define QK_FWD_PASSES 6
 #define QK_BWD_PASSES 12
 #define QK_BWD_PER_CU 2
+#define QK_SLICE_GROUPS (1 << 22)                // workgroups to a launch: a grid's threads are counted in 32 bits
 #define QK_ANGLES 1024                           // pairs of a workgroup's rows whose cosines and sines LDS holds
 
 struct QkSide {
@@ -43,7 +44,7 @@ struct QkArgs {
   QkSide s[2];                                   // q, k
   const int *places;                             // position of each row, or 0: (row mod T) + pos
   double log2_base;
-  int64_t rows;
+  int64_t rows, first;                           // all rows, and the first of this launch
   int T, pos, hd;
   float eps;
 };
@@ -121,7 +122,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_fwd_k(QkArgs A, QkPlan P) {
   const int sub = lane / LPH, li = min(lane % LPH, P.lq - 1);
   const bool mine = lane % LPH < P.lq;
   const float invd = 1.0f / (float)A.hd;
-  const int64_t row0 = (int64_t)blockIdx.x * P.R;
+  const int64_t row0 = A.first + (int64_t)blockIdx.x * P.R;
   const int nr = (int)min((int64_t)P.R, A.rows - row0);
   const int nq = nr * A.s[0].H, nk = nr * A.s[1].H, nqw = (nq + UPW - 1) / UPW, nw = nqw + (nk + UPW - 1) / UPW;
   shared_gains(A, L);
@@ -353,7 +354,7 @@ static int qk_check(gt_ctx *ctx, const char *who, int rows, int T, int Hq, int H
   GT_REQUIRE(ctx, rows >= 0 && T >= 1 && Hq >= 1 && Hkv >= 1 && q && wq && k && wk, "%s: bad arguments (rows %d, T %d, heads %d and %d)", who, rows,
              T, Hq, Hkv);
   GT_REQUIRE(ctx, hd >= 2 && hd % 2 == 0 && hd <= QK_MAX_HD, "%s: head size %d is not an even number up to %d", who, hd, QK_MAX_HD);
-  GT_REQUIRE(ctx, base > 0, "%s: the rotation's base must be positive", who);
+  GT_REQUIRE(ctx, base > 0 && base <= 1.7976931348623157e308, "%s: the rotation's base must be positive and finite", who);
   GT_REQUIRE(ctx, places || rows % T == 0, "%s: rows %d is not a whole number of sequences of %d", who, rows, T);
   const int64_t nq = (int64_t)Hq * hd, nk = (int64_t)Hkv * hd;
   GT_REQUIRE(ctx, ldq >= nq && ldk >= nk && ldqo >= nq && ldko >= nk, "%s: a row stride is less than its row (%lld and %lld elements)", who,
@@ -366,6 +367,7 @@ static int qk_bwd(gt_ctx *ctx, const char *who, int rows, int T, int Hq, int Hkv
                   int64_t ldq, gt_buf wq, gt_buf gq, int64_t ldgq, int rot_q, gt_buf dq, int acc_q, gt_buf part_q, gt_buf k, int64_t ldk, gt_buf wk,
                   gt_buf gk, int64_t ldgk, int rot_k, gt_buf dk, int acc_k, gt_buf part_k) {
   GT_REQUIRE(ctx, gq && gk && (gq | gk | dq | dk) % 4 == 0, "%s: a gradient is missing or not aligned to its elements", who);
+  GT_REQUIRE(ctx, !(dq && dq == dk), "%s: dq and dk are the same buffer", who);
   QkArgs A;
   memset(&A, 0, sizeof A);
   A.s[0] = {P<float>(q), P<float>(wq), P<float>(gq), acc_q ? P<float>(dq) : nullptr, P<float>(dq), P<float>(part_q), ldq, ldgq, Hq, rot_q != 0};
@@ -393,6 +395,7 @@ int gt_qk_norm_rope_fwd(gt_ctx *ctx, int rows, int T, int Hq, int Hkv, int hd, f
   GT_ENTER(ctx);
   if (qk_check(ctx, "gt_qk_norm_rope_fwd", rows, T, Hq, Hkv, hd, base, places, q, ldq, wq, k, ldk, wk, ldqo, ldko)) return 1;
   GT_REQUIRE(ctx, qo && ko && (qo | ko) % 4 == 0, "gt_qk_norm_rope_fwd: an output is missing or not aligned to its elements");
+  GT_REQUIRE(ctx, qo != ko, "gt_qk_norm_rope_fwd: the two outputs are the same buffer");
   if (rows == 0) return 0;
   ProfScope ps(ctx, "qknorm.rope", 8.0 * rows * (Hq + Hkv) * hd);
   QkArgs A;
@@ -404,10 +407,13 @@ int gt_qk_norm_rope_fwd(gt_ctx *ctx, int rows, int T, int Hq, int Hkv, int hd, f
   A.rows = rows; A.T = T; A.pos = pos; A.hd = hd; A.eps = eps;
   if (qk_vec(hd, A.s[0], A.s[1])) {
     const QkPlan plan = qk_plan(hd, (int)std::min<int64_t>(qk_rows_at_once(Hq + Hkv, hd, QK_FWD_PASSES), std::max(1, rows / ctx->num_cu)), Hq, Hkv);
-    const unsigned nb = (unsigned)cdiv(rows, plan.R);
+    const int64_t most = (int64_t)QK_SLICE_GROUPS * plan.R;
+    for (A.first = 0; A.first < rows; A.first += most) {
+      const unsigned nb = (unsigned)cdiv(std::min<int64_t>(most, rows - A.first), plan.R);
 #define CALL(L) hipLaunchKernelGGL((qk_norm_rope_fwd_k<L>), dim3(nb), dim3(256), 0, ctx->stream, A, plan)
-    QK_LPH(hd, CALL);
+      QK_LPH(hd, CALL);
 #undef CALL
+    }
   } else {
     const unsigned nb = (unsigned)std::min<int64_t>(rows, (int64_t)ctx->num_cu * 8);
     hipLaunchKernelGGL(qk_norm_rope_fwd_gen, dim3(nb), dim3(256), 0, ctx->stream, A);

@@ -245,7 +245,7 @@ int gt_rope_pair(gt_ctx *ctx, int rows, int T, int hd, double base, int pos, int
  * dwk) is skipped. dq (dk) may be gq (gk) itself where strides agree and acc is 0. Results do not depend on timing.
  * The gain sums go through the context's workspace; gt_qk_norm_rope_bwd_parts instead leaves gt_qk_norm_rope_parts_rows partial rows
  * of hd floats per side in the caller's buffers (0: that side's sums are not wanted), for gt_colsum_group to add when they are
- * needed: the same bits, and no allocation under a graph capture. */
+ * needed: the same bits, and no allocation. */
 int gt_qk_norm_rope_fwd(gt_ctx *ctx, int rows, int T, int Hq, int Hkv, int hd, float eps, double base, int pos, gt_buf places,
                         gt_buf q, int64_t ldq, gt_buf wq, gt_buf qo, int64_t ldqo,
                         gt_buf k, int64_t ldk, gt_buf wk, gt_buf ko, int64_t ldko);
@@ -337,7 +337,7 @@ int gt_adamw_destroy(gt_ctx *ctx, gt_adamw *opt);
  * the block and the place in it determine: pass another seed each step (the step number will do); the same seed gives the
  * same bits. Gradients and weights are FP32, the update uses the moments before they are rounded, and the norm for the
  * clip is summed in 64 bits. A moment that is not finite is held as NaN. The handle is gt_adamw's: gt_adamw_grad_norm and
- * gt_adamw_destroy take it, gt_adamw_step does not. With the clip and without it a step allocates nothing and can be captured.
+ * gt_adamw_destroy take it, gt_adamw_step does not. A step allocates nothing. No two of the w, m, r and e buffers may overlap.
  *   gt_adamw8_read:  the moments of tensor i as FP32 values, m and v = r^2 (0: not wanted)
  *   gt_adamw8_write: the states of tensor i from FP32 moments, rounded to nearest; what gt_adamw8_read gave comes back unchanged */
 int gt_adamw8_create(gt_ctx *ctx, int n, const gt_buf *w, const gt_buf *g, const gt_buf *m, const gt_buf *r, const gt_buf *e,

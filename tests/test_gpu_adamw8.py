@@ -325,6 +325,19 @@ def test_moments_out_and_in_again(gpu, n):
         half = np.full(n, 32768.0)
         check_state(m.astype(np.float64), mc, em, half, False, "m")
         check_state(np.sqrt(v.astype(np.float64)), rc, er, half, True, "r")
+        # second moments that are none: below zero and not finite are held as NaN and leave their neighbours' exponent alone, -0 is 0
+        if n > 260:
+            v2 = v.copy()
+            v2[[1, 5, 258]] = -4e4, np.inf, -0.0
+            gpu.write_state_buffer(bv, v2)
+            G.check(G.L.lib.gt_adamw8_write(gpu.ctx, G.h, 1, bm, bv))
+            _, rc2, _, er2 = G.states(1)
+            assert rc2[1] & 0x7F == 0x7F and rc2[5] & 0x7F == 0x7F and rc2[258] == 0
+            same = np.ones(n, bool)
+            same[[1, 5, 258]] = False
+            if er2[0] == er[0] and er2[1] == er[1]:
+                assert np.array_equal(rc2[same], rc[same])
+            assert np.all(E4M3[rc2[same] & 0x7F] <= 448)
         # half an e4m3 step is 2^-4 of the value, or 2^-10 units where e4m3 is denormal
         got = decode(mc, em)
         assert np.all(np.abs(got - m) <= np.maximum(2.0 ** -4 * np.abs(m), 2.0 ** -10 * 2.0 ** np.repeat(em.astype(float), BLK)[:n]) * (1 + 8 * U))
@@ -376,11 +389,17 @@ def test_refusals(gpu):
     one = lambda v: (L.buf * 1)(v)  # noqa: E731
     h = C.c_void_p()
 
-    def create(w=b, g=b, m=b, r=b, e=b, size=4):
+    def create(w=b, g=b + 1024, m=b + 2048, r=b + 2304, e=b + 3072, size=4):
         L.check(gpu.ctx, lib.gt_adamw8_create(gpu.ctx, 1, one(w), one(g), one(m), one(r), one(e), (C.c_int64 * 1)(size), B1, B2, AEPS, 0.0, 1.0, C.byref(h)), "create")
-    for kw, match in ((dict(w=0), "null buffer"), (dict(e=0), "null buffer"), (dict(size=-1), "negative size"), (dict(g=b + 2), "not aligned"), (dict(e=b + 1), "not aligned")):
+    for kw, match in ((dict(w=0), "null buffer"), (dict(e=0), "null buffer"), (dict(size=-1), "negative"), (dict(size=(1 << 40) + 1), "more than 2.40"), (dict(g=b + 2), "not aligned"), (dict(e=b + 1), "not aligned")):
         with pytest.raises(L.HipError, match=match):
             create(**kw)
+    for kw in (dict(m=b + 8), dict(r=b + 2050), dict(e=b + 2048), dict(w=b + 2048)):
+        with pytest.raises(L.HipError, match="overlap"):
+            create(**kw)
+    two = (L.buf * 2)(b, b)
+    assert lib.gt_adamw8_create(gpu.ctx, 2, two, two, (L.buf * 2)(b + 64, b + 128), (L.buf * 2)(b + 192, b + 256), (L.buf * 2)(b + 320, b + 384), (C.c_int64 * 2)(4, 4),
+                                B1, B2, AEPS, 0.0, 1.0, C.byref(h)) != 0 and "overlap" in lib.gt_last_error(gpu.ctx).decode()
     assert lib.gt_adamw8_create(gpu.ctx, 1, None, one(b), one(b), one(b), one(b), (C.c_int64 * 1)(4), B1, B2, AEPS, 0.0, 1.0, C.byref(h)) != 0
     create()
     refused = lambda rc, match: (rc != 0 and match in lib.gt_last_error(gpu.ctx).decode()) or pytest.fail(match)  # noqa: E731

@@ -368,11 +368,11 @@ def test_partial_rows_and_column_sums_give_the_same_bits(gpu, bufs, hd):
 @pytest.mark.gpu
 def test_no_rows(gpu, bufs):
     L = mod("lib")
-    b = bufs.put(np.ones(64, np.float32))
+    b, d = bufs.put(np.ones(64, np.float32)), bufs.put(np.ones(64, np.float32))
     dwq, dwk = bufs.put(np.ones(64, np.float32)), bufs.put(np.ones(64, np.float32))
-    L.check(gpu.ctx, L.lib.gt_qk_norm_rope_fwd(gpu.ctx, 0, 1, 1, 1, 64, EPS, 1e4, 0, 0, b, 64, b, b, 64, b, 64, b, b, 64), "fwd")
-    L.check(gpu.ctx, L.lib.gt_qk_norm_rope_bwd(gpu.ctx, 0, 1, 1, 1, 64, EPS, 1e4, 0, 0, b, 64, b, b, 64, 1, b, 0, dwq, 0, b, 64, b, b, 64, 1, b, 0, dwk, 1), "bwd")
-    assert np.all(gpu.read_state_buffer(b, 64) == 1) and np.all(gpu.read_state_buffer(dwq, 64) == 0) and np.all(gpu.read_state_buffer(dwk, 64) == 1)
+    L.check(gpu.ctx, L.lib.gt_qk_norm_rope_fwd(gpu.ctx, 0, 1, 1, 1, 64, EPS, 1e4, 0, 0, b, 64, b, b, 64, b, 64, b, d, 64), "fwd")
+    L.check(gpu.ctx, L.lib.gt_qk_norm_rope_bwd(gpu.ctx, 0, 1, 1, 1, 64, EPS, 1e4, 0, 0, b, 64, b, b, 64, 1, b, 0, dwq, 0, b, 64, b, b, 64, 1, d, 0, dwk, 1), "bwd")
+    assert np.all(gpu.read_state_buffer(b, 64) == 1) and np.all(gpu.read_state_buffer(d, 64) == 1) and np.all(gpu.read_state_buffer(dwq, 64) == 0) and np.all(gpu.read_state_buffer(dwk, 64) == 1)
 
 
 @pytest.mark.gpu
@@ -403,23 +403,44 @@ def test_offsets_past_32_bits(gpu, bufs):
 
 
 @pytest.mark.gpu
+def test_more_workgroups_than_one_launch_takes(gpu, bufs):
+    """A row to a workgroup and more rows than 2^22: the second launch goes on where the first ended."""
+    L = mod("lib")
+    Hq, hd, rows = 48, 64, (1 << 22) + 5
+    ld = Hq * hd
+    big, bk = bufs.raw(rows * ld * 4), bufs.raw(rows * hd * 4)
+    at = [0, 1, (1 << 22) - 1, 1 << 22, (1 << 22) + 1, rows - 1]
+    q, k, wq, wk, _, _ = inputs(len(at), Hq, 1, hd, 17)
+    for i, r in enumerate(at):
+        gpu.write_state_buffer(big + r * ld * 4, q[i])
+        gpu.write_state_buffer(bk + r * hd * 4, k[i])
+    L.check(gpu.ctx, L.lib.gt_qk_norm_rope_fwd(gpu.ctx, rows, rows, Hq, 1, hd, EPS, 1e4, 0, 0, big, ld, bufs.put(wq), big, ld, bk, hd, bufs.put(wk), bk, hd), "fwd")
+    cs = angles(len(at), 1, hd, 1e4, 0, places=at)
+    for x, w, b, n in ((q, wq, big, Hq), (k, wk, bk, 1)):
+        want, size = ref_fwd(x, w, cs)
+        got = np.stack([gpu.read_state_buffer(b + r * n * hd * 4, n * hd).reshape(n, hd) for r in at])
+        assert np.all(np.abs(got - want) <= 24 * U * size)
+
+
+@pytest.mark.gpu
 def test_refusals(gpu, bufs):
     L = mod("lib")
     b = bufs.put(np.ones(4096, np.float32))
-    ok = dict(rows=4, T=2, Hq=2, Hkv=1, hd=8, eps=EPS, base=1e4, pos=0, places=0, q=b, ldq=16, wq=b, qo=b, ldqo=16, k=b, ldk=8, wk=b, ko=b, ldko=8)
+    ok = dict(rows=4, T=2, Hq=2, Hkv=1, hd=8, eps=EPS, base=1e4, pos=0, places=0, q=b, ldq=16, wq=b, qo=b, ldqo=16, k=b, ldk=8, wk=b, ko=b + 1024, ldko=8)
     fwd = lambda **kw: L.check(gpu.ctx, L.lib.gt_qk_norm_rope_fwd(gpu.ctx, *{**ok, **kw}.values()), "fwd")  # noqa: E731
     for kw, match in ((dict(rows=-1), "bad arguments"), (dict(T=0), "bad arguments"), (dict(Hq=0), "bad arguments"), (dict(Hkv=0), "bad arguments"),
                       (dict(q=0), "bad arguments"), (dict(wk=0), "bad arguments"), (dict(hd=7), "head size 7"), (dict(hd=0), "head size 0"),
-                      (dict(hd=1026, ldq=4096, ldk=4096, ldqo=4096, ldko=4096), "even number up to 1024"), (dict(base=0.0), "base must be positive"),
+                      (dict(hd=1026, ldq=4096, ldk=4096, ldqo=4096, ldko=4096), "even number up to 1024"), (dict(base=0.0), "base must be positive"), (dict(base=float("inf")), "positive and finite"), (dict(base=float("nan")), "positive and finite"),
+                      (dict(ko=b), "same buffer"),
                       (dict(T=3), "whole number of sequences"), (dict(ldq=15), "row stride"), (dict(ldko=7), "row stride"), (dict(ldk=-8), "row stride"),
-                      (dict(k=b + 2), "aligned to its elements"), (dict(qo=0), "an output is missing"), (dict(ko=b + 1), "an output is missing or not aligned"),
+                      (dict(k=b + 2), "aligned to its elements"), (dict(qo=0), "an output is missing"), (dict(ko=b + 1025), "an output is missing or not aligned"),
                       (dict(places=b + 2), "aligned to its elements")):
         with pytest.raises(L.HipError, match=match):
             fwd(**kw)
     okb = dict(rows=4, T=2, Hq=2, Hkv=1, hd=8, eps=EPS, base=1e4, pos=0, places=0, q=b, ldq=16, wq=b, gq=b, ldgq=16, rot_q=1, dq=b, acc_q=0, dwq=b, acc_wq=0,
-               k=b, ldk=8, wk=b, gk=b, ldgk=8, rot_k=1, dk=b, acc_k=0, dwk=b + 256, acc_wk=0)
+               k=b, ldk=8, wk=b, gk=b, ldgk=8, rot_k=1, dk=b + 1024, acc_k=0, dwk=b + 256, acc_wk=0)
     bwd = lambda **kw: L.check(gpu.ctx, L.lib.gt_qk_norm_rope_bwd(gpu.ctx, *{**okb, **kw}.values()), "bwd")  # noqa: E731
-    for kw, match in ((dict(gq=0), "a gradient is missing"), (dict(gk=b + 2), "a gradient is missing or not aligned"), (dict(dwk=b), "one and the same"),
+    for kw, match in ((dict(gq=0), "a gradient is missing"), (dict(gk=b + 2), "a gradient is missing or not aligned"), (dict(dwk=b), "one and the same"), (dict(dk=b), "dq and dk are the same"),
                       (dict(ldgk=4), "row stride"), (dict(hd=9), "head size 9"), (dict(T=3), "whole number of sequences")):
         with pytest.raises(L.HipError, match=match):
             bwd(**kw)
