@@ -1344,8 +1344,10 @@ class HipBackend:
             """t's rotation (input tensor, parameters) when its backward can ride this attention's write-backs: t is a
             rotation's output that only this attention has read and whose gradient nobody has touched."""
             te = self._entries.get(t)
-            if (not self.fuse_rope_bwd or not scores or te is None or te.rope_of is None or te.consumers != 1 or te.grad_init
-                    or te.grad_src or te.keep_grad or te.grad or hd % 8 or id(t) in self._pend_dx):
+            if not self.fuse_rope_bwd or not scores or te is None or te.rope_of is None or te.consumers != 1 or hd % 8 or id(t) in self._pend_dx:
+                return None
+            # an unrotated gradient that an earlier backward over this graph left here is added to as one
+            if (te.grad_init or te.grad_src or te.keep_grad or te.grad) and not te.grad_unrotated:
                 return None
             src, par = te.rope_of
             if par[0] != T or par[1] != hd:

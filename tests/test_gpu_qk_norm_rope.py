@@ -539,6 +539,55 @@ def test_two_consumers_keep_the_rotated_gradient(gpu):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T", [128, 40])
+def test_two_backwards_over_one_graph(gpu, T):
+    """Gradients of intermediates accumulate over backward passes, as the four calls' do: with the rotation undone by the attention (T = 128)
+    and by the op itself."""
+    ag = mod("autograd")
+    Hq, Hkv, hd = 2, 1, 64
+    got = []
+    for fused in (True, False):
+        rs = np.random.RandomState(24)
+        n = lambda *s: ag.Tensor(rs.standard_normal(s).astype(np.float32), list(s), True)  # noqa: E731
+        q, k, v, wq, wk = n(T, Hq * hd), n(T, Hkv * hd), n(T, Hkv * hd), n(hd), n(hd)
+        up = rs.standard_normal(T * Hq * hd)
+        gpu.install()
+        try:
+            if fused:
+                qo, ko = ag.qk_norm_rope(q, k, wq, wk, T, Hq, Hkv, hd, EPS, 1e4)
+            else:
+                qn, kn = ag.rms_norm_heads(q, wq, T, Hq, hd, EPS), ag.rms_norm_heads(k, wk, T, Hkv, hd, EPS)
+                # scaled by one: a consumer between the rotation and the attention keeps its backward a launch of its own
+                qo, ko = ag.scale(ag.rope(qn, T, Hq, hd, 1e4), 1.0), ag.scale(ag.rope(kn, T, Hkv, hd, 1e4), 1.0)
+            out = ag.attention(qo, ko, v, T, Hq, Hkv, hd)
+            backward_from(gpu, ag, out, up)
+            first = [gpu.read_state_buffer(gpu.buffers_for(t)["grad"], t.size).copy() for t in (q, k, wq, wk)]
+            gpu.sync([])
+        finally:
+            gpu.uninstall()
+        got.append(first + [t.grad.copy() for t in (q, k, v, wq, wk)])
+    for a, b in zip(*got):
+        assert np.linalg.norm(a.astype(np.float64) - b) <= 1e-6 * np.linalg.norm(b)
+    # the same graph differentiated twice: every leaf's gradient is its first one three times over, intermediates having added up,
+    # but v's, which only the attention itself writes, twice
+    rs = np.random.RandomState(24)
+    n = lambda *s: ag.Tensor(rs.standard_normal(s).astype(np.float32), list(s), True)  # noqa: E731
+    q, k, v, wq, wk = n(T, Hq * hd), n(T, Hkv * hd), n(T, Hkv * hd), n(hd), n(hd)
+    up = rs.standard_normal(T * Hq * hd)
+    gpu.install()
+    try:
+        qo, ko = ag.qk_norm_rope(q, k, wq, wk, T, Hq, Hkv, hd, EPS, 1e4)
+        out = ag.attention(qo, ko, v, T, Hq, Hkv, hd)
+        for _ in range(2):
+            backward_from(gpu, ag, out, up)
+        gpu.sync([])
+    finally:
+        gpu.uninstall()
+    for t, once, times in ((q, got[0][4], 3), (k, got[0][5], 3), (v, got[0][6], 2), (wq, got[0][7], 3), (wk, got[0][8], 3)):
+        assert np.linalg.norm(t.grad.astype(np.float64) - times * once.astype(np.float64)) <= 1e-6 * times * np.linalg.norm(once)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("name,T", [("qwen3", 21), ("gemma3", 21), ("gemma3-window", 128), ("qwen3-hd128", 128)])
 @pytest.mark.parametrize("recompute", [False, True])
 def test_models_call_it(gpu, ref, name, T, recompute):
