@@ -373,15 +373,22 @@ int gt_adamw8_create(gt_ctx *ctx, int n, const gt_buf *w, const gt_buf *g, const
     }
   }
   o->nchunks = (int)ch.size();
+  // one allocation: scale and norm, the norm's partial sums, the chunk table
+  const size_t head = 256 + NORM8_GROUPS * sizeof(double), bytes = head + ch.size() * sizeof(Chunk8);
   const float one[2] = {1.0f, 0.0f};
-  hipError_t err;
-  if ((err = hipMalloc((void **)&o->chunks8, std::max<size_t>(1, ch.size()) * sizeof(Chunk8))) != hipSuccess ||
-      (err = hipMalloc((void **)&o->sums8, NORM8_GROUPS * sizeof(double))) != hipSuccess || (err = hipMalloc((void **)&o->scale, 8)) != hipSuccess ||
-      (!ch.empty() && (err = hipMemcpy(o->chunks8, ch.data(), ch.size() * sizeof(Chunk8), hipMemcpyHostToDevice)) != hipSuccess) ||
-      (err = hipMemcpy(o->scale, one, 8, hipMemcpyHostToDevice)) != hipSuccess) {
+  hipError_t err = hipMalloc(&o->block8, bytes);
+  if (err == hipSuccess) {
+    char *at = static_cast<char *>(o->block8);
+    o->scale = reinterpret_cast<float *>(at);
+    o->sums8 = reinterpret_cast<double *>(at + 256);
+    o->chunks8 = reinterpret_cast<Chunk8 *>(at + head);
+    err = hipMemcpy(o->scale, one, sizeof one, hipMemcpyHostToDevice);
+    if (err == hipSuccess && !ch.empty()) err = hipMemcpy(o->chunks8, ch.data(), ch.size() * sizeof(Chunk8), hipMemcpyHostToDevice);
+  }
+  if (err != hipSuccess) {
     (void)hipGetLastError();
     adamw_release(o);
-    GT_FAIL(ctx, "gt_adamw8_create: setting up the chunk tables failed: %s", hipGetErrorString(err));
+    GT_FAIL(ctx, "gt_adamw8_create: setting up the chunk table failed: %s", hipGetErrorString(err));
   }
   ctx->adamws.insert(o);
   *out = o;

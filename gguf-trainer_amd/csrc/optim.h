@@ -21,6 +21,7 @@ struct gt_adamw {
   float *partial = nullptr;     // [nchunks]
   float *scale = nullptr;       // [2]: clip scale, grad norm
   bool bits8 = false;
+  void *block8 = nullptr;       // the one allocation behind scale, sums8 and chunks8 of a group with 8-bit moments
   Chunk8 *chunks8 = nullptr;
   double *sums8 = nullptr;      // partial sums of squares, one per workgroup of the norm's kernel
   std::vector<Tensor8> tensors8;

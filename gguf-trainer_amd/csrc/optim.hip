@@ -312,10 +312,9 @@ static int group_alloc(gt_ctx *ctx, MuonGroup &G) {
 void adamw_release(gt_adamw *o) {
   if (o->chunks) (void)hipFree(o->chunks);
   if (o->ptrs) (void)hipFree(o->ptrs);
-  if (o->chunks8) (void)hipFree(o->chunks8);
-  if (o->sums8) (void)hipFree(o->sums8);
   if (o->partial) (void)hipFree(o->partial);
-  if (o->scale) (void)hipFree(o->scale);
+  if (o->block8) (void)hipFree(o->block8);
+  else if (o->scale) (void)hipFree(o->scale);
   delete o;
 }
 static void muon_release(gt_ctx *ctx, gt_muon *o) {

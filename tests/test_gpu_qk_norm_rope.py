@@ -496,6 +496,16 @@ def test_one_op_equals_the_four_calls(gpu, T, B, Hq, Hkv, hd):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T,Hq,Hkv,hd", [(9, 2, 1, 16), (7, 2, 2, 6)])
+def test_device_gradients_equal_device_differences(gpu, ref, T, Hq, Hkv, hd):
+    """The recipe (and its bounds) that every op of the backend goes through, on the op with an attention behind it."""
+    from test_gpu_fd import R, fd_case
+    g = R(ref, 77)
+    fd_case(gpu, ref, [g(T, Hq * hd), g(T, Hkv * hd), g(T, Hkv * hd), 1 + 0.3 * g(hd), 1 + 0.3 * g(hd)],
+            lambda ag, q, k, v, wq, wk: ag.attention(*ag.qk_norm_rope(q, k, wq, wk, T, Hq, Hkv, hd, EPS, 1e4, 2), v, T, Hq, Hkv, hd), "qk_norm_rope")
+
+
+@pytest.mark.gpu
 def test_frozen_leaves_an_unused_output_and_positions(gpu):
     full = graph(gpu, True, 37, 2, 4, 2, 64, 21)
     for frozen in (("wq",), ("wk", "wq"), ("q",), ("k", "wk"), ("q", "k")):        # what is left out changes no bit of the rest
