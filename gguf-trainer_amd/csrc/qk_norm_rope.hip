@@ -6,8 +6,8 @@
 //   backward  gy = R^T g (or g, where the rotation has been undone already);  S = sum(gy w x);
 //             dx = r w gy - x r^3 S / hd;  dw = sum over rows and heads of gy x r                        (h = hd / 2)
 //
-// Bound by memory: 8 bytes per element forward, 12 backward, about 20 operations. 16384 rows of 16 + 8 heads of 128 take 65.6 us
-// forward (6.1 TB/s) and 98 us backward (6.2 TB/s; the gain sums are another launch of 4 us); a large copy reaches 5.0.
+// Bound by memory: 8 bytes per element forward, 12 backward, about 20 operations. 16384 rows of 16 + 8 heads of 128 take 63.4 us
+// forward (6.35 TB/s) and 98 us backward (6.2 TB/s; the gain sums are another launch of 4 us); a large copy reaches 5.0.
 // A head is handled by LPH lanes of one wavefront, each holding four elements of the lower half and the four of the upper half
 // they are rotated with, so a pair never leaves its lane and the row sums are the only exchange. r is formed again in the
 // backward (its row is in registers anyway) instead of being stored. Every row is read once and far from its next use: all
