@@ -374,7 +374,7 @@ def qk_norm_rope(q, k, q_weight, k_weight, T: int, Hq: int, Hkv: int, hd: int, e
         raise ValueError(f"qkNormRope: {rows} rows are not a whole number of sequences of {T}")
     be = _be()
     # one tensor in both places takes two gradients, which the one-launch backward would write at once
-    if hasattr(be, "qk_norm_rope") and q is not k and q_weight is not k_weight and hd % 2 == 0 and hd <= 1024:
+    if hasattr(be, "qk_norm_rope") and q is not k and q_weight is not k_weight and hd % 2 == 0 and hd <= 1024 and max(Hq, Hkv) <= 32768:
         return be.qk_norm_rope(q, k, q_weight, k_weight, T, Hq, Hkv, hd, eps, base, pos_offset, positions)
     if positions is not None:
         raise ValueError("qkNormRope: positions need the fused op (even head size up to 1024, q and k distinct)")

@@ -22,6 +22,7 @@
 typedef float v4f __attribute__((ext_vector_type(4)));
 
 #define QK_MAX_HD 1024                           // the generic kernels keep a head's gain sums in LDS, one copy per wavefront
+#define QK_MAX_HEADS 32768                       // of one side: a head's row is found by a 32-bit multiplication
 #define QK_VEC_HD 512                            // 64 lanes of eight elements
 // Measured on 16384 rows of 16 + 8 heads of 128 and of 10 + 2 heads of 64 (and 32768 rows of the former, backward):
 //   forward: 4 to 6 passes (one row of the first) 65.6 and 19.5 us, 12 passes 68.5 and 20.3, 24 passes 71.2 and 20.1
@@ -87,17 +88,19 @@ template <int LPH> __device__ __forceinline__ float head_sum(float v) {
   return v;
 }
 __device__ __forceinline__ float sum4(v4f t) { return (t[0] + t[1]) + (t[2] + t[3]); }
-// 1 / sqrt(t): the hardware's and one Newton step
+// 1 / sqrt(t): the hardware's, which takes no denormals, and one Newton step
 __device__ __forceinline__ float inv_root(float t) {
-  const float y = __builtin_amdgcn_rsqf(t);
-  return __builtin_fmaf(0.5f * y, __builtin_fmaf(-t * y, y, 1.0f), y);
+  const bool tiny = t < 1.17549435e-38f;
+  t = tiny ? t * 1.84467441e19f : t;             // 2^64
+  float y = __builtin_amdgcn_rsqf(t);
+  y = __builtin_fmaf(0.5f * y, __builtin_fmaf(-t * y, y, 1.0f), y);
+  return tiny ? y * 4294967296.0f : y;
 }
 
 // What a workgroup keeps of its rows and the gains: [row][pair] cosines and sines, [side][hd].
-struct QkShared { float c[QK_ANGLES], s[QK_ANGLES], w[2][QK_VEC_HD]; };
+struct alignas(16) QkShared { float c[QK_ANGLES], s[QK_ANGLES], w[2][QK_VEC_HD]; };
 
-// A workgroup takes R rows at a time (R * hd/2 <= 256 angles, one per thread). Its wavefronts go through the rows' heads of q and
-// then of k, 64 / LPH heads at a time, so that all of a wavefront is on one side and what differs between the sides is scalar.
+// A workgroup takes R rows at a time (R * hd/2 <= QK_ANGLES). Its wavefronts go through the rows' heads of q and then of k, 64 / LPH heads at a time, so that all of a wavefront is on one side and what differs between the sides is scalar.
 struct QkPlan { int R, half, lq; unsigned mq, mk; };
 __device__ __forceinline__ void shared_gains(const QkArgs &A, QkShared &L) {
   for (int i = threadIdx.x; i < 2 * A.hd; i += 256) L.w[i >= A.hd][i >= A.hd ? i - A.hd : i] = i >= A.hd ? A.s[1].w[i - A.hd] : A.s[0].w[i];
@@ -331,7 +334,7 @@ static int qk_rows_at_once(int heads, int hd, int passes) {
   return (int)std::max<int64_t>(1, std::min<int64_t>(QK_ANGLES / (hd / 2), cdiv((int64_t)passes * (WAVE / QK_LPH_OF(hd)), heads)));
 }
 static QkPlan qk_plan(int hd, int R, int Hq, int Hk) {
-  // heads are fewer than 2^15 per group of rows, so that u / H is the high word of 2 u * ceil(2^31 / H)
+  // u / H is the high word of 2 u * ceil(2^31 / H) where u * H < 2^31; u is below H + QK_BWD_PASSES * 16 here, H at most 2^15
   return {R, hd / 2, hd / 8, (unsigned)((0x80000000ull + Hq - 1) / Hq), (unsigned)((0x80000000ull + Hk - 1) / Hk)};
 }
 // A backward call's workgroups, one partial row of gain sums each, of the vector and of the generic kernel alike; and the rows that
@@ -356,6 +359,7 @@ static int qk_check(gt_ctx *ctx, const char *who, int rows, int T, int Hq, int H
   GT_REQUIRE(ctx, hd >= 2 && hd % 2 == 0 && hd <= QK_MAX_HD, "%s: head size %d is not an even number up to %d", who, hd, QK_MAX_HD);
   GT_REQUIRE(ctx, base > 0 && base <= 1.7976931348623157e308, "%s: the rotation's base must be positive and finite", who);
   GT_REQUIRE(ctx, places || rows % T == 0, "%s: rows %d is not a whole number of sequences of %d", who, rows, T);
+  GT_REQUIRE(ctx, Hq <= QK_MAX_HEADS && Hkv <= QK_MAX_HEADS, "%s: %d and %d heads are more than %d", who, Hq, Hkv, QK_MAX_HEADS);
   const int64_t nq = (int64_t)Hq * hd, nk = (int64_t)Hkv * hd;
   GT_REQUIRE(ctx, ldq >= nq && ldk >= nk && ldqo >= nq && ldko >= nk, "%s: a row stride is less than its row (%lld and %lld elements)", who,
              (long long)nq, (long long)nk);
@@ -368,6 +372,7 @@ static int qk_bwd(gt_ctx *ctx, const char *who, int rows, int T, int Hq, int Hkv
                   gt_buf gk, int64_t ldgk, int rot_k, gt_buf dk, int acc_k, gt_buf part_k) {
   GT_REQUIRE(ctx, gq && gk && (gq | gk | dq | dk) % 4 == 0, "%s: a gradient is missing or not aligned to its elements", who);
   GT_REQUIRE(ctx, !(dq && dq == dk), "%s: dq and dk are the same buffer", who);
+  GT_REQUIRE(ctx, !(dq == gq && ldq != ldgq) && !(dk == gk && ldk != ldgk), "%s: in place the strides have to be the same", who);
   QkArgs A;
   memset(&A, 0, sizeof A);
   A.s[0] = {P<float>(q), P<float>(wq), P<float>(gq), acc_q ? P<float>(dq) : nullptr, P<float>(dq), P<float>(part_q), ldq, ldgq, Hq, rot_q != 0};
@@ -396,6 +401,7 @@ int gt_qk_norm_rope_fwd(gt_ctx *ctx, int rows, int T, int Hq, int Hkv, int hd, f
   if (qk_check(ctx, "gt_qk_norm_rope_fwd", rows, T, Hq, Hkv, hd, base, places, q, ldq, wq, k, ldk, wk, ldqo, ldko)) return 1;
   GT_REQUIRE(ctx, qo && ko && (qo | ko) % 4 == 0, "gt_qk_norm_rope_fwd: an output is missing or not aligned to its elements");
   GT_REQUIRE(ctx, qo != ko, "gt_qk_norm_rope_fwd: the two outputs are the same buffer");
+  GT_REQUIRE(ctx, !(qo == q && ldqo != ldq) && !(ko == k && ldko != ldk), "gt_qk_norm_rope_fwd: in place the strides have to be the same");
   if (rows == 0) return 0;
   ProfScope ps(ctx, "qknorm.rope", 8.0 * rows * (Hq + Hkv) * hd);
   QkArgs A;

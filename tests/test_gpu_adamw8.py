@@ -297,6 +297,40 @@ def test_seeds(gpu):
 
 
 @pytest.mark.gpu
+def test_two_groups_on_two_contexts_at_once(gpu):
+    """Groups of two contexts (two streams) stepped in turn without waiting: each does what it does alone."""
+    hb = mod("hip_backend")
+    sizes = [300000, 5000, 17]
+    other = hb.HipBackend(0, streams=1)
+    try:
+        def groups(a, b):
+            rs = np.random.RandomState(6)
+            w = [rs.standard_normal(n).astype(np.float32) for n in sizes]
+            G = [Group(be, w, clip=1.0) for be in (a, b)]
+            for i, x in enumerate(G):
+                x.grads([rs.standard_normal(n) * (i + 1) for n in sizes])
+            return G
+        A, B = groups(gpu, other)
+        for t in range(1, 6):
+            A.step(t)
+            B.step(t)
+        other.sync([])
+        both = [[a for i in range(3) for a in (x.weights(i), *x.states(i))] for x in (A, B)]
+        A.free()
+        B.free()
+        C_, D = groups(gpu, gpu)
+        for x in (C_, D):
+            for t in range(1, 6):
+                x.step(t)
+        alone = [[a for i in range(3) for a in (x.weights(i), *x.states(i))] for x in (C_, D)]
+        C_.free()
+        D.free()
+        assert all(np.array_equal(a, b) for p, q in zip(both, alone) for a, b in zip(p, q))
+    finally:
+        other.destroy()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("n", [1, 300, 70001])
 def test_moments_out_and_in_again(gpu, n):
     """What read gives, write takes back without a change; other values come in rounded to the nearest."""

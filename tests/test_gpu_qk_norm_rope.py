@@ -2,7 +2,7 @@
 
 Bounds, from the number of roundings in 32 bits (u = 2^-24, half a step): a row's sum of squares passes at most 20 of them (squares, a
 lane's own sum of up to 16 products, six exchanges), mean, eps, root and reciprocal five more, of which the root halves the
-first: r is off by at most 15 u, y = x r w by 17 u, cos and sin by one each, a rotated element by 24 u (|y_j| + |y_{j+h}|). The
+first: r is off by at most 15 u, y = x r w by 17 u, cos and sin by two each, a rotated element by 24 u (|y_j| + |y_{j+h}|). The
 backward's first term w g r takes the rotation's 4 and r's 15: 24 u; its second, x r^3 S / hd, 3 * 15 from r^3 and at most 20
 from S: 72 u of the sum of absolute products. A gain sum is at most 20 u per term, a lane's chain of at most H terms, 64 lane
 groups, and 1024 partial rows summed as 64 by 16: (20 + H + 64 + 64 + 16) u of the sum of absolute terms."""
@@ -178,7 +178,7 @@ def inputs(rows, Hq, Hkv, hd, seed):
 SHAPES = [(1, 1, 1, 1, 2, 0), (5, 5, 3, 1, 6, 0), (7, 7, 2, 2, 10, 3), (300, 100, 5, 5, 8, 0), (9, 9, 2, 1, 16, 1), (66, 33, 4, 4, 24, 0),
           (130, 65, 4, 4, 48, 0), (127, 127, 10, 2, 64, 0), (12, 4, 4, 2, 80, 7), (66, 33, 9, 3, 96, 0), (1, 1, 16, 8, 128, 100000),
           (1030, 515, 16, 8, 128, 0), (20, 10, 4, 2, 160, 0), (40, 20, 8, 4, 256, 0), (6, 3, 2, 1, 512, 0), (4, 2, 3, 1, 514, 0), (3, 3, 1, 1, 1024, 11),
-          (2, 1, 7, 1, 4, 16000000)]
+          (2, 1, 7, 1, 4, 16000000), (3, 3, 32768, 5, 8, 0), (2, 2, 1, 1001, 16, 0), (5, 5, 333, 20000, 6, 0)]
 
 
 def run_fwd(gpu, bufs, shape, seed, pad=(0, 0), shift=0, places=None, base=1e6):
@@ -258,6 +258,23 @@ def test_forward_in_place_and_rows_apart(gpu, bufs, hd):
         with np.errstate(invalid="ignore"):
             want, size = ref_fwd(x, w, cs)
         assert np.all(np.abs(got - want)[ok] <= 24 * U * size[ok])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 256, 6])
+def test_rows_too_small_for_their_squares(gpu, bufs, hd):
+    """Without an eps, rows whose mean square is a denormal: each square is off by at most 2^-150, and they are above 1e-41 on the average,
+    so r is off by less than 2^-150 / 1e-41 / 2 < 4e-5 of itself."""
+    L = mod("lib")
+    q, k, wq, wk, _, _ = inputs(4, 2, 1, hd, 18)
+    q, k = (1e-20 * q / np.sqrt((q * q).mean(axis=2, keepdims=True))).astype(np.float32), (3e-20 * k / np.sqrt((k * k).mean(axis=2, keepdims=True))).astype(np.float32)
+    oq, ok = bufs.raw(q.nbytes), bufs.raw(k.nbytes)
+    L.check(gpu.ctx, L.lib.gt_qk_norm_rope_fwd(gpu.ctx, 4, 4, 2, 1, hd, 0.0, 1e4, 0, 0, bufs.put(q), 2 * hd, bufs.put(wq), oq, 2 * hd, bufs.put(k), hd, bufs.put(wk), ok, hd),
+            "fwd")
+    cs = angles(4, 4, hd, 1e4, 0)
+    for x, w, b, n in ((q, wq, oq, 2), (k, wk, ok, 1)):
+        want, size = ref_fwd(x, w, cs, 0.0)
+        assert np.all(np.abs(gpu.read_state_buffer(b, x.size).reshape(4, n, hd) - want) <= (4e-5 + 24 * U) * size)
 
 
 def run_bwd(gpu, bufs, shape, seed, rot=(1, 1), acc=(0, 0), accw=(0, 0), want=("dq", "dwq", "dk", "dwk"), pad=(0, 0), shift=0, places=None, base=1e6,
@@ -366,6 +383,34 @@ def test_partial_rows_and_column_sums_give_the_same_bits(gpu, bufs, hd):
 
 
 @pytest.mark.gpu
+def test_two_contexts_at_once(gpu, bufs):
+    """Calls on two contexts (two streams) overlap; each has its own workspace for the gain sums. The second one's inputs are made on the
+    first one's stream, which it waits for on the device."""
+    L, hb = mod("lib"), mod("hip_backend")
+    rows, Hq, Hkv, hd = 6000, 4, 2, 64
+    q, k, wq, wk, gq, gk = inputs(rows, Hq, Hkv, hd, 19)
+    ins = [bufs.put(a) for a in (q, k, wq, wk, gq, gk)]
+    other = hb.HipBackend(0, streams=1)
+    try:
+        out = [[bufs.raw(n) for n in (q.nbytes, k.nbytes, hd * 4, hd * 4)] for _ in range(2)]
+        L.check(gpu.ctx, L.lib.gt_stream_mark(gpu.ctx), "mark")
+        L.check(other.ctx, L.lib.gt_stream_wait(other.ctx, gpu.ctx), "wait")
+        bq, bk, bwq, bwk, bgq, bgk = ins
+        for _ in range(3):
+            for c, (dq, dk, dwq, dwk) in ((gpu.ctx, out[0]), (other.ctx, out[1])):
+                L.check(c, L.lib.gt_qk_norm_rope_bwd(c, rows, 2000, Hq, Hkv, hd, EPS, 1e6, 0, 0, bq, Hq * hd, bwq, bgq, Hq * hd, 1, dq, 0, dwq, 0,
+                                                     bk, Hkv * hd, bwk, bgk, Hkv * hd, 1, dk, 0, dwk, 0), "bwd")
+        L.check(other.ctx, L.lib.gt_sync(other.ctx), "sync")
+        for a, b, n in zip(*out, (q.size, k.size, hd, hd)):
+            assert np.array_equal(gpu.read_state_buffer(a, n), gpu.read_state_buffer(b, n))
+        cs = angles(rows, 2000, hd, 1e6, 0)
+        dx, _, off, _ = ref_bwd(q, wq, gq, cs, 1)
+        assert np.all(np.abs(gpu.read_state_buffer(out[1][0], q.size).reshape(rows, Hq, hd) - dx) <= off + 2 * U * np.abs(dx))
+    finally:
+        other.destroy()
+
+
+@pytest.mark.gpu
 def test_no_rows(gpu, bufs):
     L = mod("lib")
     b, d = bufs.put(np.ones(64, np.float32)), bufs.put(np.ones(64, np.float32))
@@ -431,7 +476,8 @@ def test_refusals(gpu, bufs):
     for kw, match in ((dict(rows=-1), "bad arguments"), (dict(T=0), "bad arguments"), (dict(Hq=0), "bad arguments"), (dict(Hkv=0), "bad arguments"),
                       (dict(q=0), "bad arguments"), (dict(wk=0), "bad arguments"), (dict(hd=7), "head size 7"), (dict(hd=0), "head size 0"),
                       (dict(hd=1026, ldq=4096, ldk=4096, ldqo=4096, ldko=4096), "even number up to 1024"), (dict(base=0.0), "base must be positive"), (dict(base=float("inf")), "positive and finite"), (dict(base=float("nan")), "positive and finite"),
-                      (dict(ko=b), "same buffer"),
+                      (dict(ko=b), "same buffer"), (dict(Hq=32769, ldq=1 << 20, ldqo=1 << 20), "heads are more than 32768"),
+                      (dict(qo=b, ldqo=20), "strides have to be the same"),
                       (dict(T=3), "whole number of sequences"), (dict(ldq=15), "row stride"), (dict(ldko=7), "row stride"), (dict(ldk=-8), "row stride"),
                       (dict(k=b + 2), "aligned to its elements"), (dict(qo=0), "an output is missing"), (dict(ko=b + 1025), "an output is missing or not aligned"),
                       (dict(places=b + 2), "aligned to its elements")):
@@ -441,6 +487,7 @@ def test_refusals(gpu, bufs):
                k=b, ldk=8, wk=b, gk=b, ldgk=8, rot_k=1, dk=b + 1024, acc_k=0, dwk=b + 256, acc_wk=0)
     bwd = lambda **kw: L.check(gpu.ctx, L.lib.gt_qk_norm_rope_bwd(gpu.ctx, *{**okb, **kw}.values()), "bwd")  # noqa: E731
     for kw, match in ((dict(gq=0), "a gradient is missing"), (dict(gk=b + 2), "a gradient is missing or not aligned"), (dict(dwk=b), "one and the same"), (dict(dk=b), "dq and dk are the same"),
+                      (dict(ldgq=20), "strides have to be the same"),
                       (dict(ldgk=4), "row stride"), (dict(hd=9), "head size 9"), (dict(T=3), "whole number of sequences")):
         with pytest.raises(L.HipError, match=match):
             bwd(**kw)
