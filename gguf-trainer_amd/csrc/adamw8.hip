@@ -44,6 +44,7 @@ typedef GLOBAL unsigned char gbyte;
 
 struct Adam8H { float b1, b2, omb1, omb2, eps, wd, lr, ibc1, rbc2; unsigned key; };
 
+// The random bits: a multiply-xorshift mixer, two rounds of it for a block's key and one from there for each element.
 __host__ __device__ __forceinline__ unsigned mix1(unsigned x) {
   x ^= x >> 16;
   x *= 0x21F0AAADu;

@@ -107,12 +107,14 @@ class AdamWHip:
         if self.state_bits == 8:
             out = {"m": [], "v": [], "t": self.t}
             bm, bv = self._moment_pair()
-            for i, p in enumerate(self.params):
-                check(self.gpu.ctx, lib.gt_adamw8_read(self.gpu.ctx, self._h, i, bm, bv), "gt_adamw8_read")
-                out["m"].append(self.gpu.read_state_buffer(bm, p.size))
-                out["v"].append(self.gpu.read_state_buffer(bv, p.size))
-            self.gpu.free_state_buffer(bm)
-            self.gpu.free_state_buffer(bv)
+            try:
+                for i, p in enumerate(self.params):
+                    check(self.gpu.ctx, lib.gt_adamw8_read(self.gpu.ctx, self._h, i, bm, bv), "gt_adamw8_read")
+                    out["m"].append(self.gpu.read_state_buffer(bm, p.size))
+                    out["v"].append(self.gpu.read_state_buffer(bv, p.size))
+            finally:
+                self.gpu.free_state_buffer(bm)
+                self.gpu.free_state_buffer(bv)
             return out
         return {"m": [self.gpu.read_state_buffer(b, p.size) for b, p in zip(self._m, self.params)],
                 "v": [self.gpu.read_state_buffer(b, p.size) for b, p in zip(self._v, self.params)], "t": self.t}
@@ -125,12 +127,14 @@ class AdamWHip:
                 if np.asarray(m).size != p.size or np.asarray(v).size != p.size:
                     raise ValueError(f"adam state size mismatch: {np.asarray(m).size}/{np.asarray(v).size} vs {p.size}")
             bm, bv = self._moment_pair()
-            for i, (m, v) in enumerate(zip(s["m"], s["v"])):
-                self.gpu.write_state_buffer(bm, np.asarray(m, dtype=np.float32))
-                self.gpu.write_state_buffer(bv, np.asarray(v, dtype=np.float32))
-                check(self.gpu.ctx, lib.gt_adamw8_write(self.gpu.ctx, self._h, i, bm, bv), "gt_adamw8_write")
-            self.gpu.free_state_buffer(bm)
-            self.gpu.free_state_buffer(bv)
+            try:
+                for i, (m, v) in enumerate(zip(s["m"], s["v"])):
+                    self.gpu.write_state_buffer(bm, np.asarray(m, dtype=np.float32))
+                    self.gpu.write_state_buffer(bv, np.asarray(v, dtype=np.float32))
+                    check(self.gpu.ctx, lib.gt_adamw8_write(self.gpu.ctx, self._h, i, bm, bv), "gt_adamw8_write")
+            finally:
+                self.gpu.free_state_buffer(bm)
+                self.gpu.free_state_buffer(bv)
             self.t = int(s["t"])
             return
         for b, a in zip(self._m, s["m"]):
