@@ -113,7 +113,7 @@ class _Entry:
         self.sgrad = None           # parameters: {stream: [accumulator, written?]} of the streams other than the first
         self.rope_of = None         # a rotation's output: (input tensor, (T, hd, base, pos)); of a norm and rotation in one: (None, ...)
         self.rope_fused = False     # an attention backward wrote the rotation's input gradient itself: the rotation's closure has nothing to do
-        self.grad_unrotated = False # an attention backward left the gradient of the rows before the rotation here
+        self.grad_unrotated = False # an attention backward left the gradient of the rows before the rotation here (see _turn_back)
 
 
 class HipBackend:
@@ -575,9 +575,21 @@ class HipBackend:
         if e.stream != self._cur and not e.external:
             check(self._ctxs[e.stream], lib.gt_sync(self._ctxs[e.stream]), "gt_sync")
 
-    def _gdst(self, t: Tensor) -> tuple:
+    def _turn_back(self, t: Tensor, e: _Entry):
+        """t's gradient is about to be used as what it is, that of the rotated rows, but an attention's backward has left that of the
+        rows before the rotation: rotate it. Into another buffer, and the old one stays taken until the streams are idle, since
+        held-back launches know buffers by their address."""
+        _, (T, hd, base, pos) = e.rope_of
+        new = self._acquire(e.nbytes, e.stream)
+        check(self._ctx, lib.gt_rope(self._ctx, t.shape[0], T, t.shape[1] // hd, hd, base, pos, 0, e.grad, new, 0), "rope")
+        self._scratch.append((e.grad, e.nbytes, e.stream))
+        e.grad = new
+        e.grad_unrotated = False
+
+    def _gdst(self, t: Tensor, unrotated: bool = False) -> tuple:
         """(gradient buffer, acc) for a backward kernel about to contribute to t's gradient;
-        (0, 0) when t takes no gradient (a frozen parameter)."""
+        (0, 0) when t takes no gradient (a frozen parameter). unrotated: the kernel writes the gradient of the rows before t's
+        rotation, and t's entry says so from here on."""
         self._flush()
         if self._pend_dx:
             self._flush_dx(t)       # products held back for this gradient go first: the order of its writers is kept
@@ -611,6 +623,10 @@ class HipBackend:
         if e.grad_src:
             check(self._ctx, lib.gt_d2d(self._ctx, e.grad, e.grad_src, e.nbytes), "gt_d2d")
             e.grad_src = 0
+        if unrotated:
+            e.grad_unrotated = True
+        elif e.grad_unrotated:
+            self._turn_back(t, e)
         acc = 1 if e.grad_init else 0
         e.grad_init = True
         return e.grad, acc
@@ -651,8 +667,9 @@ class HipBackend:
                 e.grad_src = 0
         self._aliased = []
 
-    def _gsrc(self, t: Tensor) -> int:
-        """Gradient buffer of an op output inside its backward closure."""
+    def _gsrc(self, t: Tensor, unrotated: bool = False) -> int:
+        """Gradient buffer of an op output inside its backward closure. unrotated: the closure looks at the entry's grad_unrotated and
+        takes either form."""
         self._flush()
         if self._pend_dx:
             self._flush_dx(t)
@@ -668,6 +685,8 @@ class HipBackend:
                                "gradient buffers, so this backward would read pool garbage")
         self._bw_seen = True
         self._same_stream(e)
+        if e.grad_unrotated and not unrotated:
+            self._turn_back(t, e)
         if e.grad_src:
             return e.grad_src       # handed on by an add's backward and not written since: read it where it is
         if e.grad == 0 or not e.grad_init:
@@ -694,6 +713,9 @@ class HipBackend:
             e.grad = self._acquire(e.nbytes, e.stream)
             check(self._ctx, lib.gt_memset0(self._ctx, e.grad, e.nbytes), "gt_memset0")
             self.grad_clears_issued += 1
+        if e.grad_unrotated:
+            self._turn_back(t, e)
+            self._barrier0()
         return {"data": e.data, "grad": e.grad}
 
     def release(self, tensors):
@@ -767,6 +789,7 @@ class HipBackend:
         check(self._ctx, lib.gt_h2d(self._ctx, e.grad, t.grad.ctypes.data_as(C.c_void_p), e.nbytes), "gt_h2d")
         e.grad_init = True
         e.grad_src = 0
+        e.grad_unrotated = False
 
     def create_state_buffer(self, nbytes: int) -> int:
         out = c_buf()
@@ -1293,7 +1316,7 @@ class HipBackend:
         wants_q, wants_k = qw.requires_grad, kw.requires_grad
 
         def bw():
-            gq, gk = self._gsrc(qo), self._gsrc(ko)
+            gq, gk = self._gsrc(qo, True), self._gsrc(ko, True)
             rq, rk = (0 if self._entries[t].grad_unrotated else 1 for t in (qo, ko))
             dq, aq = self._gdst(q)
             dk, ak = self._gdst(k)
@@ -1366,13 +1389,12 @@ class HipBackend:
                 rk = None                           # two different rotations: one table per call
             if rq or rk:
                 par = (rq or rk)[1]
-                dq, aq = self._gdst(rq[0] if rq else q)
-                dk, ak = self._gdst(rk[0] if rk else k)
+                # the rotation's input gradient; of a norm and rotation in one, the output's own, before the rotation
+                dq, aq = self._gdst(rq[0], rq[0] is q) if rq else self._gdst(q)
+                dk, ak = self._gdst(rk[0], rk[0] is k) if rk else self._gdst(k)
                 dv, av = self._gdst(v)
                 for t, r in ((q, rq), (k, rk)):
-                    if r and r[0] is t:
-                        self._entries[t].grad_unrotated = True
-                    elif r:
+                    if r and r[0] is not t:
                         self._entries[t].rope_fused = True
                 check(self._ctx, lib.gt_attn_bwd_scores_rope(self._ctx, B, T, Hq, Hkv, hd, window, qd, kd, vd, od, g, lse, scores,
                                                              par[2], par[3], 1 if rq else 0, 1 if rk else 0,
