@@ -30,7 +30,7 @@ class Tensor:
     """autograd.ts:20-51. Host arrays are allocated on first touch: an intermediate that lives on
     the device only never pays for a host copy. They are authoritative only after backend.sync()."""
 
-    __slots__ = ("shape", "requires_grad", "_backward", "_prev", "seq", "_data", "_grad", "_dev", "__weakref__")
+    __slots__ = ("shape", "requires_grad", "_backward", "_prev", "seq", "_data", "_grad", "_dev", "_outs", "__weakref__")
 
     def __init__(self, data, shape, requires_grad=False):
         global _created
@@ -42,6 +42,7 @@ class Tensor:
         self._data = data
         self._grad = None
         self._dev = None                # a device backend's record for this tensor: (owner key, record)
+        self._outs = None               # an op with several outputs: [(output, the inputs that output alone is made of)] (see _topo)
         self.requires_grad = requires_grad
         self._backward = _noop
         self._prev = []
@@ -111,6 +112,21 @@ def param(shape, std, rng) -> Tensor:
 
 
 def _topo(root, seen):
+    """The tensors below root, each after everything it was made of. An op with several outputs is a node of its own between them and its
+    inputs; the inputs of outputs that root does not depend on are left out, as they are where every output is an op."""
+    topo = _walk(root, seen, {})
+    cut = {}
+    while True:
+        parts = [t for t in topo if t._outs is not None and id(t) not in cut and any(id(o) not in seen for o, _ in t._outs)]
+        if not parts:
+            return topo
+        for t in parts:
+            cut[id(t)] = [p for o, ins in t._outs if id(o) in seen for p in ins]
+        seen.difference_update([id(t) for t in topo])
+        topo = _walk(root, seen, cut)
+
+
+def _walk(root, seen, cut):
     topo = []
     if id(root) in seen:
         return topo
@@ -118,9 +134,10 @@ def _topo(root, seen):
     stack = [(root, 0)]
     while stack:
         t, i = stack.pop()
-        if i < len(t._prev):
+        prev = t._prev if t._outs is None else cut.get(id(t), t._prev)
+        if i < len(prev):
             stack.append((t, i + 1))
-            p = t._prev[i]
+            p = prev[i]
             if id(p) not in seen:
                 seen.add(id(p))
                 stack.append((p, 0))

@@ -1299,29 +1299,35 @@ class HipBackend:
         return out
 
     def qk_norm_rope(self, q, k, qw, kw, T, Hq, Hkv, hd, eps, base, pos_offset=0, positions=None):
-        """Both head norms and both rotations as one launch, and their backward as another. The outputs are two tensors with
-        one closure: k's output names q's as its predecessor, so q's closure runs when both gradients are complete."""
+        """Both head norms and both rotations as one launch, and their backward as another. The op is a node of its own behind its two
+        outputs, so its closure runs when both gradients are complete; the outputs' closures note which of them a backward has
+        come through. The other side, whose gradient may be an earlier backward's, gets nothing."""
         self._op_begin(q, k, qw, kw)
         rows = q.shape[0]
         base, pos_offset = float(base), int(pos_offset)
         qd, kd, qwd, kwd = self._data(q), self._data(k), self._data(qw), self._data(kw)
         places = 0 if positions is None else self._upload(np.ascontiguousarray(positions, dtype=np.int32))
-        qo, eq = self._make_out([rows, Hq * hd], [q, k, qw, kw])
-        ko, ek = self._make_out([rows, Hkv * hd], [qo])
+        op, _ = self._make_out([1], [q, k, qw, kw], alloc=False)
+        qo, eq = self._make_out([rows, Hq * hd], [op])
+        ko, ek = self._make_out([rows, Hkv * hd], [op])
+        op._outs = [(qo, [q, qw]), (ko, [k, kw])]
         if positions is None:
             eq.rope_of = ek.rope_of = (None, (T, hd, base, pos_offset))
         ldq, ldk = Hq * hd, Hkv * hd
         check(self._ctx, lib.gt_qk_norm_rope_fwd(self._ctx, rows, T, Hq, Hkv, hd, eps, base, pos_offset, places, qd, ldq, qwd, eq.data, ldq,
                                                  kd, ldk, kwd, ek.data, ldk), "qkNormRope")
         wants_q, wants_k = qw.requires_grad, kw.requires_grad
+        reached = set()
 
         def bw():
             gq, gk = self._gsrc(qo, True), self._gsrc(ko, True)
             rq, rk = (0 if self._entries[t].grad_unrotated else 1 for t in (qo, ko))
-            dq, aq = self._gdst(q)
-            dk, ak = self._gdst(k)
-            dwq, awq = self._gdst(qw) if wants_q else (0, 0)
-            dwk, awk = self._gdst(kw) if wants_k else (0, 0)
+            on_q, on_k = "q" in reached, "k" in reached
+            reached.clear()
+            dq, aq = self._gdst(q) if on_q else (0, 0)
+            dk, ak = self._gdst(k) if on_k else (0, 0)
+            dwq, awq = self._gdst(qw) if wants_q and on_q else (0, 0)
+            dwk, awk = self._gdst(kw) if wants_k and on_k else (0, 0)
             nparts = C.c_int(0)
             if self.defer_norm_dw and (dwq or dwk):
                 check(self._ctx, lib.gt_qk_norm_rope_parts_rows(self._ctx, rows, Hq, Hkv, hd, C.byref(nparts)), "qkNormRope.bwd")
@@ -1337,7 +1343,9 @@ class HipBackend:
             check(self._ctx, lib.gt_qk_norm_rope_bwd(self._ctx, rows, T, Hq, Hkv, hd, eps, base, pos_offset, places, qd, ldq, qwd, gq, ldq, rq, dq, aq,
                                                      dwq, awq, kd, ldk, kwd, gk, ldk, rk, dk, ak, dwk, awk), "qkNormRope.bwd")
 
-        qo._backward = bw
+        qo._backward = lambda: reached.add("q")
+        ko._backward = lambda: reached.add("k")
+        op._backward = bw
         return qo, ko
 
     def attention(self, q, k, v, T, Hq, Hkv, hd, window=0):
