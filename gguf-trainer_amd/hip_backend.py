@@ -92,7 +92,7 @@ class _EntryMap:
 class _Entry:
     __slots__ = ("data", "grad", "nbytes", "external", "grad_init", "lazy_act", "consumers", "fused_uses",
                  "region", "keep_grad", "extra", "needs_grad", "lazy_lin", "grad_src", "stream", "sgrad", "rope_of", "rope_fused",
-                 "grad_unrotated")
+                 "grad_unrotated", "rope_out")
 
     def __init__(self, nbytes, external):
         self.data = 0
@@ -112,7 +112,9 @@ class _Entry:
         self.stream = 0             # the stream whose launches produce and consume this tensor (its buffers come from that stream's pool)
         self.sgrad = None           # parameters: {stream: [accumulator, written?]} of the streams other than the first
         self.rope_of = None         # a rotation's output: (input tensor, (T, hd, base, pos)); of a norm and rotation in one: (None, ...)
-        self.rope_fused = False     # an attention backward wrote the rotation's input gradient itself: the rotation's closure has nothing to do
+        self.rope_fused = 0         # an attention backward wrote the rotation's input gradient itself: 1 until the rotation's closure has come by, which
+                                    # then has nothing to do; 2 from there on (see _restore_rotated)
+        self.rope_out = None        # the rotation's output whose gradient this gradient is, rotated back, and nothing else so far
         self.grad_unrotated = False # an attention backward left the gradient of the rows before the rotation here (see _turn_back)
 
 
@@ -586,6 +588,26 @@ class HipBackend:
         e.grad = new
         e.grad_unrotated = False
 
+    def _restore_rotated(self, t: Tensor, e: _Entry):
+        """An attention's backward has passed over t, a rotation's output, and left the gradient in the rotation's input alone. Gradients add up over
+        backward passes, so before t's is used, or the input's becomes more than that, t gets its own: the input's rotated."""
+        src, (T, hd, base, pos) = e.rope_of
+        se = self._entries.get(src)
+        if se is None:
+            raise RuntimeError("backward over a graph whose rotation's input was released")
+        e.rope_fused, se.rope_out = 0, None
+        if e.grad == 0:
+            e.grad = self._acquire(e.nbytes, e.stream)
+        check(self._ctx, lib.gt_rope(self._ctx, t.shape[0], T, t.shape[1] // hd, hd, base, pos, 0, se.grad, e.grad, 0), "rope")
+        e.grad_init = True
+
+    def _settle_rotated(self, e: _Entry):
+        """The gradient of a rotation's input is about to be written by somebody else."""
+        t, e.rope_out = e.rope_out, None
+        te = self._entries.get(t)
+        if te is not None and te.rope_fused:        # a released output needs nothing any more
+            self._restore_rotated(t, te)
+
     def _gdst(self, t: Tensor, unrotated: bool = False) -> tuple:
         """(gradient buffer, acc) for a backward kernel about to contribute to t's gradient;
         (0, 0) when t takes no gradient (a frozen parameter). unrotated: the kernel writes the gradient of the rows before t's
@@ -627,6 +649,10 @@ class HipBackend:
             e.grad_unrotated = True
         elif e.grad_unrotated:
             self._turn_back(t, e)
+        if e.rope_fused:
+            self._restore_rotated(t, e)
+        if e.rope_out is not None:
+            self._settle_rotated(e)
         acc = 1 if e.grad_init else 0
         e.grad_init = True
         return e.grad, acc
@@ -687,6 +713,8 @@ class HipBackend:
         self._same_stream(e)
         if e.grad_unrotated and not unrotated:
             self._turn_back(t, e)
+        if e.rope_fused:
+            self._restore_rotated(t, e)
         if e.grad_src:
             return e.grad_src       # handed on by an add's backward and not written since: read it where it is
         if e.grad == 0 or not e.grad_init:
@@ -715,6 +743,9 @@ class HipBackend:
             self.grad_clears_issued += 1
         if e.grad_unrotated:
             self._turn_back(t, e)
+            self._barrier0()
+        if e.rope_fused:
+            self._restore_rotated(t, e)
             self._barrier0()
         return {"data": e.data, "grad": e.grad}
 
@@ -784,6 +815,13 @@ class HipBackend:
         e = self._entries.get(t)
         if e is None:
             raise RuntimeError("seed_grad_from_host: tensor has no device buffers")
+        if e.rope_out is not None:
+            self._settle_rotated(e)
+        if e.rope_fused:
+            e.rope_fused = 0
+            se = self._entries.get(e.rope_of[0])
+            if se is not None:
+                se.rope_out = None
         if e.grad == 0:
             e.grad = self._acquire(e.nbytes, e.stream)
         check(self._ctx, lib.gt_h2d(self._ctx, e.grad, t.grad.ctypes.data_as(C.c_void_p), e.nbytes), "gt_h2d")
@@ -1288,7 +1326,8 @@ class HipBackend:
 
         def bw():           # the two backward rotations are never neighbours in the tape's order (k's linear sits between them)
             oe = self._entries.get(out)
-            if oe is not None and oe.rope_fused:
+            if oe is not None and oe.rope_fused == 1:
+                oe.rope_fused = 2
                 return      # the attention that consumed this rotation wrote x's gradient in its own write-back
             g = self._gsrc(out)
             dx, acc = self._gdst(x)
@@ -1373,9 +1412,11 @@ class HipBackend:
 
         def rope_source(t):
             """t's rotation (input tensor, parameters) when its backward can ride this attention's write-backs: t is a
-            rotation's output that only this attention has read and whose gradient nobody has touched."""
+            rotation's output that only this attention has read and whose gradient nobody has touched, and so is the rotation's input
+            (a leaf's gradient outlives the graph: not that)."""
             te = self._entries.get(t)
-            if not self.fuse_rope_bwd or not scores or te is None or te.rope_of is None or te.consumers != 1 or hd % 8 or id(t) in self._pend_dx:
+            if (not self.fuse_rope_bwd or not scores or te is None or te.rope_of is None or te.consumers != 1 or te.rope_fused or hd % 8
+                    or id(t) in self._pend_dx):
                 return None
             # an unrotated gradient that an earlier backward over this graph left here is added to as one
             if (te.grad_init or te.grad_src or te.keep_grad or te.grad) and not te.grad_unrotated:
@@ -1386,7 +1427,7 @@ class HipBackend:
             if src is None:
                 return t, par                       # its own closure does the norm's part and skips the rotation's
             se = self._entries.get(src)
-            if se is None or (se.external and not src.requires_grad):
+            if se is None or se.external or se.consumers != 1 or se.grad or se.grad_src:
                 return None
             return src, par
 
@@ -1403,7 +1444,8 @@ class HipBackend:
                 dv, av = self._gdst(v)
                 for t, r in ((q, rq), (k, rk)):
                     if r and r[0] is not t:
-                        self._entries[t].rope_fused = True
+                        self._entries[t].rope_fused = 1
+                        self._entries[r[0]].rope_out = t
                 check(self._ctx, lib.gt_attn_bwd_scores_rope(self._ctx, B, T, Hq, Hkv, hd, window, qd, kd, vd, od, g, lse, scores,
                                                              par[2], par[3], 1 if rq else 0, 1 if rk else 0,
                                                              dq, aq, dk, ak, dv, av), "attention.bwd")
