@@ -88,12 +88,12 @@ template <int LPH> __device__ __forceinline__ float head_sum(float v) {
   return v;
 }
 __device__ __forceinline__ float sum4(v4f t) { return (t[0] + t[1]) + (t[2] + t[3]); }
-// 1 / sqrt(t): the hardware's, which takes no denormals, and one Newton step
+// 1 / sqrt(t): the hardware's, which takes no denormals, and one Newton step; zero for infinity, where the step would make 0 * infinity
 __device__ __forceinline__ float inv_root(float t) {
   const bool tiny = t < 1.17549435e-38f;
   t = tiny ? t * 1.84467441e19f : t;             // 2^64
   float y = __builtin_amdgcn_rsqf(t);
-  y = __builtin_fmaf(0.5f * y, __builtin_fmaf(-t * y, y, 1.0f), y);
+  if (t < __builtin_inff()) y = __builtin_fmaf(0.5f * y, __builtin_fmaf(-t * y, y, 1.0f), y);
   return tiny ? y * 4294967296.0f : y;
 }
 
