@@ -204,10 +204,11 @@ __global__ __launch_bounds__(256) void qk_norm_rope_bwd_k(QkArgs A, QkPlan P) {
       const float ss = head_sum<LPH>(mine ? sum4(a * a + b * b) : 0.f);
       const float dot = head_sum<LPH>(mine ? sum4(ga * wa * a + gb * wb * b) : 0.f);
       const float r = inv_root(ss * invd + A.eps);
-      const float k2 = r * r * r * dot * invd;
+      // x r^3 S / hd as (x r) (r S / hd r), about as large as the result: the cube by itself would leave FP32 at rows below 1e-13
+      const float k1 = r * dot * invd * r;
       if (S.o && live) {
-        __builtin_nontemporal_store(wa * ga * r - a * k2 + oa, reinterpret_cast<v4f *>(S.o + xo) + li);
-        __builtin_nontemporal_store(wb * gb * r - b * k2 + ob, reinterpret_cast<v4f *>(S.o + xo + half) + li);
+        __builtin_nontemporal_store(wa * ga * r - a * r * k1 + oa, reinterpret_cast<v4f *>(S.o + xo) + li);
+        __builtin_nontemporal_store(wb * gb * r - b * r * k1 + ob, reinterpret_cast<v4f *>(S.o + xo + half) + li);
       }
       const float rl = u < n ? r : 0.f;          // a head past the last one adds nothing
       const v4f ta = u < n ? ga * a * rl : v4f{0, 0, 0, 0}, tb = u < n ? gb * b * rl : v4f{0, 0, 0, 0};
@@ -285,7 +286,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_bwd_gen(QkArgs A) {
       }
       ss = wave_sum(ss);
       dot = wave_sum(dot);
-      const float r = 1.0f / sqrtf(ss / (float)A.hd + A.eps), k2 = r * r * r * dot / (float)A.hd;
+      const float r = 1.0f / sqrtf(ss / (float)A.hd + A.eps), k1 = r * dot / (float)A.hd * r;
       float *dw = acc + (size_t)(wave * 2 + side) * A.hd;
       for (int j = lane; j < half; j += WAVE) {
         const float c = S.rot ? cs[j].x : 1.f, sn = S.rot ? cs[j].y : 0.f;
@@ -295,8 +296,8 @@ __global__ __launch_bounds__(256) void qk_norm_rope_bwd_gen(QkArgs A) {
         dw[j + half] += gb * xb * r;
         if (S.o) {
           const float oa = S.old ? S.old[xo + j] : 0.f, ob = S.old ? S.old[xo + j + half] : 0.f;
-          S.o[xo + j] = S.w[j] * ga * r - xa * k2 + oa;
-          S.o[xo + j + half] = S.w[j + half] * gb * r - xb * k2 + ob;
+          S.o[xo + j] = S.w[j] * ga * r - xa * r * k1 + oa;
+          S.o[xo + j + half] = S.w[j + half] * gb * r - xb * r * k1 + ob;
         }
       }
     }
