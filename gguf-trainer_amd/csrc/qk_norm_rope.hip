@@ -17,6 +17,7 @@
 // fraction of a turn with the whole turns taken off, and leaves cos and sin in LDS for every head of the row: positions may
 // be anything (a decoding batch's rows each have their own) and no table grows with them.
 #include <algorithm>
+#include <initializer_list>
 #include "common.h"
 
 typedef float v4f __attribute__((ext_vector_type(4)));
@@ -368,12 +369,52 @@ static int qk_check(gt_ctx *ctx, const char *who, int rows, int T, int Hq, int H
   return 0;
 }
 
+// Buffers of a call that it writes, and which of the others each may not share memory with: every workgroup writes while others still read.
+// A buffer is `rows` runs of n bytes, ld bytes apart (a plain one: one run).
+struct QkSpan { const char *name; uint64_t at; int64_t rows, ld, n; };
+static QkSpan qk_plain(const char *name, gt_buf at, int64_t elems) { return {name, at, 1, 0, elems * 4}; }
+static QkSpan qk_rows(const char *name, gt_buf at, int rows, int64_t ld, int64_t elems) { return {name, at, rows, ld * 4, elems * 4}; }
+static bool qk_same(const QkSpan &a, const QkSpan &b) { return a.at == b.at && a.n == b.n && (a.ld == b.ld || (a.rows == 1 && b.rows == 1)); }
+// Whether a run of a meets a run of b. Where the strides are the same (or one has a single run) that is a multiple k of the stride,
+// 1 - b.rows <= k <= a.rows - 1, with b.at - a.at - a.n < k ld < b.at - a.at + b.n. Rows that interleave at different strides count as meeting.
+static bool qk_meet(const QkSpan &a, const QkSpan &b) {
+  if (!a.at || !b.at || a.rows < 1 || b.rows < 1 || a.n < 1 || b.n < 1) return false;
+  typedef __int128 wide;
+  const wide ea = (wide)a.at + (wide)(a.rows - 1) * a.ld + a.n, eb = (wide)b.at + (wide)(b.rows - 1) * b.ld + b.n;
+  if (ea <= (wide)b.at || eb <= (wide)a.at) return false;
+  if (a.rows > 1 && b.rows > 1 && a.ld != b.ld) return true;
+  const wide ld = a.rows > 1 ? a.ld : b.rows > 1 ? b.ld : 1, far = (wide)b.at - (wide)a.at;
+  const wide low = far - a.n;                    // the least k with k ld above it
+  wide k = low >= 0 ? low / ld + 1 : -((-low + ld - 1) / ld) + 1;
+  k = std::max<wide>(k, 1 - (wide)b.rows);
+  return k <= (wide)a.rows - 1 && k * ld < far + b.n;
+}
+// out against everything in `others`; `self` may be out itself (in place)
+static int qk_apart(gt_ctx *ctx, const char *who, const QkSpan &out, std::initializer_list<QkSpan> self, std::initializer_list<QkSpan> others) {
+  for (const QkSpan &o : self)
+    GT_REQUIRE(ctx, qk_same(out, o) || !qk_meet(out, o), "%s: %s and %s overlap (in place they have to be the same rows)", who, out.name, o.name);
+  for (const QkSpan &o : others) GT_REQUIRE(ctx, !qk_meet(out, o), "%s: %s and %s overlap", who, out.name, o.name);
+  return 0;
+}
+
 static int qk_bwd(gt_ctx *ctx, const char *who, int rows, int T, int Hq, int Hkv, int hd, float eps, double base, int pos, gt_buf places, gt_buf q,
                   int64_t ldq, gt_buf wq, gt_buf gq, int64_t ldgq, int rot_q, gt_buf dq, int acc_q, gt_buf part_q, gt_buf k, int64_t ldk, gt_buf wk,
-                  gt_buf gk, int64_t ldgk, int rot_k, gt_buf dk, int acc_k, gt_buf part_k) {
+                  gt_buf gk, int64_t ldgk, int rot_k, gt_buf dk, int acc_k, gt_buf part_k, gt_buf dwq, gt_buf dwk) {
   GT_REQUIRE(ctx, gq && gk && (gq | gk | dq | dk) % 4 == 0, "%s: a gradient is missing or not aligned to its elements", who);
   GT_REQUIRE(ctx, !(dq && dq == dk), "%s: dq and dk are the same buffer", who);
   GT_REQUIRE(ctx, !(dq == gq && ldq != ldgq) && !(dk == gk && ldk != ldgk), "%s: in place the strides have to be the same", who);
+  const int nb = qk_bwd_groups(ctx, rows, Hq + Hkv, hd);
+  const int64_t nq = (int64_t)Hq * hd, nk = (int64_t)Hkv * hd, np = (int64_t)nb * hd;
+  const QkSpan sq = qk_rows("q", q, rows, ldq, nq), sk = qk_rows("k", k, rows, ldk, nk), sgq = qk_rows("gq", gq, rows, ldgq, nq),
+               sgk = qk_rows("gk", gk, rows, ldgk, nk), sdq = qk_rows("dq", dq, rows, ldq, nq), sdk = qk_rows("dk", dk, rows, ldk, nk),
+               swq = qk_plain("wq", wq, hd), swk = qk_plain("wk", wk, hd), sp = qk_plain("places", places, rows),
+               spq = qk_plain("parts_q", part_q, np), spk = qk_plain("parts_k", part_k, np);
+  if (qk_apart(ctx, who, sdq, {sq, sgq}, {sk, sgk, swq, swk, sp, sdk}) || qk_apart(ctx, who, sdk, {sk, sgk}, {sq, sgq, swq, swk, sp}) ||
+      qk_apart(ctx, who, spq, {}, {sq, sk, sgq, sgk, swq, swk, sp, sdq, sdk, spk}) ||
+      qk_apart(ctx, who, spk, {}, {sq, sk, sgq, sgk, swq, swk, sp, sdq, sdk})) return 1;
+  // the gain gradients are written when everything has been read
+  const QkSpan sdwq = qk_plain("dwq", dwq, hd), sdwk = qk_plain("dwk", dwk, hd);
+  if (qk_apart(ctx, who, sdwq, {}, {sdq, sdk, sdwk}) || qk_apart(ctx, who, sdwk, {}, {sdq, sdk})) return 1;
   QkArgs A;
   memset(&A, 0, sizeof A);
   A.s[0] = {P<float>(q), P<float>(wq), P<float>(gq), acc_q ? P<float>(dq) : nullptr, P<float>(dq), P<float>(part_q), ldq, ldgq, Hq, rot_q != 0};
@@ -381,7 +422,6 @@ static int qk_bwd(gt_ctx *ctx, const char *who, int rows, int T, int Hq, int Hkv
   A.places = P<const int>(places);
   A.log2_base = log2(base);
   A.rows = rows; A.T = T; A.pos = pos; A.hd = hd; A.eps = eps;
-  const int nb = qk_bwd_groups(ctx, rows, Hq + Hkv, hd);
   if (qk_vec(hd, A.s[0], A.s[1])) {
     const QkPlan plan = qk_plan(hd, qk_bwd_rows(ctx, rows, Hq + Hkv, hd), Hq, Hkv);
 #define CALL(L) hipLaunchKernelGGL((qk_norm_rope_bwd_k<L>), dim3((unsigned)nb), dim3(256), 0, ctx->stream, A, plan)
@@ -404,6 +444,10 @@ int gt_qk_norm_rope_fwd(gt_ctx *ctx, int rows, int T, int Hq, int Hkv, int hd, f
   GT_REQUIRE(ctx, qo != ko, "gt_qk_norm_rope_fwd: the two outputs are the same buffer");
   GT_REQUIRE(ctx, !(qo == q && ldqo != ldq) && !(ko == k && ldko != ldk), "gt_qk_norm_rope_fwd: in place the strides have to be the same");
   if (rows == 0) return 0;
+  const int64_t nq = (int64_t)Hq * hd, nk = (int64_t)Hkv * hd;
+  const QkSpan sq = qk_rows("q", q, rows, ldq, nq), sk = qk_rows("k", k, rows, ldk, nk), sqo = qk_rows("qo", qo, rows, ldqo, nq),
+               sko = qk_rows("ko", ko, rows, ldko, nk), swq = qk_plain("wq", wq, hd), swk = qk_plain("wk", wk, hd), sp = qk_plain("places", places, rows);
+  if (qk_apart(ctx, "gt_qk_norm_rope_fwd", sqo, {sq}, {sk, swq, swk, sp, sko}) || qk_apart(ctx, "gt_qk_norm_rope_fwd", sko, {sk}, {sq, swq, swk, sp})) return 1;
   ProfScope ps(ctx, "qknorm.rope", 8.0 * rows * (Hq + Hkv) * hd);
   QkArgs A;
   memset(&A, 0, sizeof A);
@@ -456,7 +500,7 @@ int gt_qk_norm_rope_bwd(gt_ctx *ctx, int rows, int T, int Hq, int Hkv, int hd, f
   {
     ProfScope ps(ctx, "qknorm.rope.bwd", 12.0 * rows * (Hq + Hkv) * hd);
     if (qk_bwd(ctx, "gt_qk_norm_rope_bwd", rows, T, Hq, Hkv, hd, eps, base, pos, places, q, ldq, wq, gq, ldgq, rot_q, dq, acc_q, pq, k, ldk, wk, gk,
-               ldgk, rot_k, dk, acc_k, pk)) return 1;
+               ldgk, rot_k, dk, acc_k, pk, dwq, dwk)) return 1;
   }
   gt_buf sp[2], sd[2];
   int sn[2], sw[2], sa[2], n = 0;
@@ -480,6 +524,6 @@ int gt_qk_norm_rope_bwd_parts(gt_ctx *ctx, int rows, int T, int Hq, int Hkv, int
              "gt_qk_norm_rope_bwd_parts: bad arguments (rows %d; 16-byte aligned partial rows for q, k or both)", rows);
   ProfScope ps(ctx, "qknorm.rope.bwd", 12.0 * rows * (Hq + Hkv) * hd);
   return qk_bwd(ctx, "gt_qk_norm_rope_bwd_parts", rows, T, Hq, Hkv, hd, eps, base, pos, places, q, ldq, wq, gq, ldgq, rot_q, dq, acc_q, parts_q, k,
-                ldk, wk, gk, ldgk, rot_k, dk, acc_k, parts_k);
+                ldk, wk, gk, ldgk, rot_k, dk, acc_k, parts_k, 0, 0);
 }
 }

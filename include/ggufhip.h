@@ -238,11 +238,13 @@ int gt_rope_pair(gt_ctx *ctx, int rows, int T, int hd, double base, int pos, int
  * belong to as many sequences as there are rows (one new token of each). Angles are formed in 64 bits.
  * Strides are in elements between consecutive rows: ldq / ldk of q / k and of dq / dk, ldqo / ldko of the rotated rows and ldgq / ldgk
  * of their gradients; a row's heads lie next to each other, so q and k may be slices of one wider product. qo may be q itself
- * and ko k itself (same stride). At most 32768 heads a side; hd is even and at most 1024; multiples of 8 up to 512 with 16-byte aligned buffers and strides of
+ * and ko k itself (same stride). Beyond that what a call writes may not share memory with anything else it reads or writes (the gain
+ * gradients, written last: with anything else it writes): such calls are refused, and so are rows that interleave at different strides.
+ * At most 32768 heads a side; hd is even and at most 1024; multiples of 8 up to 512 with 16-byte aligned buffers and strides of
  * whole 16-byte chunks take the vector kernels, everything else a generic one.
  * Backward: q and k are the rows before the norm (nothing is kept from the forward). rot_q (rot_k) = 1: gq (gk) is the gradient of
  * the rotated rows; 0: of the rows between norm and rotation, what gt_attn_bwd_scores_rope leaves. A destination of 0 (dq, dk, dwq,
- * dwk) is skipped. dq (dk) may be gq (gk) itself where strides agree and acc is 0. Results do not depend on timing.
+ * dwk) is skipped. dq (dk) may be gq (gk) itself where strides agree and acc is 0, or q (k) itself. Results do not depend on timing.
  * The gain sums go through the context's workspace; gt_qk_norm_rope_bwd_parts instead leaves gt_qk_norm_rope_parts_rows partial rows
  * of hd floats per side in the caller's buffers (0: that side's sums are not wanted), for gt_colsum_group to add when they are
  * needed: the same bits, and no allocation. */

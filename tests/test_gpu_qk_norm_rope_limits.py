@@ -76,3 +76,118 @@ def test_backward_of_rows_too_small_for_the_cube_of_their_root(gpu, bufs, hd, sh
         assert np.all(np.isfinite(got)) and np.all(np.abs(got - want) <= off + 2 * U * (np.abs(want) + acc * np.abs(o)))
         got = gpu.read_state_buffer(bw, hd)
         assert np.all(np.abs(got - dw) <= offw + d * (size * np.abs(x64) * r).sum(axis=(0, 1)) + 2 * U * np.abs(dw))
+
+
+# ---- which buffers may share memory -----------------------------------------------------------------------------------
+
+
+def forward_args(rows, Hq, Hkv, hd, **kw):
+    a = dict(rows=rows, T=rows, Hq=Hq, Hkv=Hkv, hd=hd, eps=EPS, base=1e4, pos=0, places=0, q=0, ldq=Hq * hd, wq=0, qo=0, ldqo=Hq * hd, k=0, ldk=Hkv * hd, wk=0, ko=0,
+             ldko=Hkv * hd)
+    return {**a, **kw}
+
+
+def backward_args(rows, Hq, Hkv, hd, **kw):
+    a = dict(rows=rows, T=rows, Hq=Hq, Hkv=Hkv, hd=hd, eps=EPS, base=1e4, pos=0, places=0, q=0, ldq=Hq * hd, wq=0, gq=0, ldgq=Hq * hd, rot_q=1, dq=0, acc_q=0, dwq=0,
+             acc_wq=0, k=0, ldk=Hkv * hd, wk=0, gk=0, ldgk=Hkv * hd, rot_k=1, dk=0, acc_k=0, dwk=0, acc_wk=0)
+    return {**a, **kw}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 6])
+def test_overlapping_buffers_are_refused(gpu, bufs, hd):  # noqa: F811
+    """What would let one workgroup write what another has still to read. Nothing is launched."""
+    L = mod("lib")
+    rows, Hq, Hkv = 40, 4, 2
+    nq, nk = rows * Hq * hd * 4, rows * Hkv * hd * 4
+    fill = lambda n: bufs.put(np.ones(n // 4, np.float32))  # noqa: E731
+    b = {m: fill(n) for m, n in dict(q=nq, k=nk, gq=nq, gk=nk, qo=nq, ko=nk, dq=nq, dk=nk).items()}
+    b.update({m: fill(4 * hd) for m in ("wq", "wk", "dwq", "dwk")})
+    at = bufs.put(np.zeros(rows, np.int32))
+    parts = [bufs.raw(1 << 22) for _ in range(2)]
+    pick = lambda *names: {m: b[m] for m in names}  # noqa: E731
+    okf = forward_args(rows, Hq, Hkv, hd, places=at, **pick("q", "k", "wq", "wk", "qo", "ko"))
+    okb = backward_args(rows, Hq, Hkv, hd, places=at, **pick("q", "k", "wq", "wk", "gq", "gk", "dq", "dk", "dwq", "dwk"))
+    fwd = lambda **kw: L.check(gpu.ctx, L.lib.gt_qk_norm_rope_fwd(gpu.ctx, *{**okf, **kw}.values()), "fwd")  # noqa: E731
+    bwd = lambda **kw: L.check(gpu.ctx, L.lib.gt_qk_norm_rope_bwd(gpu.ctx, *{**okb, **kw}.values()), "bwd")  # noqa: E731
+
+    def leave(pq, pk, **kw):
+        a = {n: v for n, v in {**okb, **kw}.items() if n not in ("dwq", "acc_wq", "dwk", "acc_wk")}
+        names = list(a)
+        i = names.index("acc_q") + 1
+        L.check(gpu.ctx, L.lib.gt_qk_norm_rope_bwd_parts(gpu.ctx, *[a[n] for n in names[:i]], pq, *[a[n] for n in names[i:]], pk), "parts")
+    fwd()
+    bwd()
+    leave(*parts)
+    gpu.sync([])
+    before = {m: gpu.read_state_buffer(x, hd) for m, x in b.items()}
+    row, head = Hkv * hd * 4, hd * 4
+    for kw in (dict(qo=b["k"]), dict(ko=b["q"]), dict(ko=b["q"] + nq - 4), dict(qo=b["q"] + 4), dict(qo=b["q"] + head), dict(ko=b["k"] + row), dict(qo=b["ko"] + nk - 4),
+               dict(ko=b["qo"] + 4 * Hq * hd), dict(qo=b["wq"]), dict(ko=b["wq"] - nk + 4), dict(qo=b["wk"]), dict(qo=at), dict(ko=at + 4 * rows - 4),
+               dict(ko=b["k"], q=b["k"], ldq=Hq * hd)):
+        with pytest.raises(L.HipError, match="overlap"):
+            fwd(**kw)
+    for kw in (dict(dq=b["gk"]), dict(dk=b["gq"]), dict(dq=b["k"]), dict(dk=b["q"]), dict(dq=b["q"] + 4), dict(dq=b["gq"] + head), dict(dk=b["dq"] + 4),
+               dict(dq=b["dk"] + nk - 4), dict(dk=b["wk"]), dict(dk=b["wq"]), dict(dq=b["wk"] - nq + 4), dict(dq=at), dict(dwq=b["dq"]), dict(dwk=b["dq"] + 8),
+               dict(dwq=b["dk"] + nk - 4), dict(dwk=b["dwq"] + 4), dict(dq=b["gq"], gk=b["gq"]), dict(dq=b["q"], k=b["q"])):
+        with pytest.raises(L.HipError, match="overlap"):
+            bwd(**kw)
+    for a in ((parts[0], parts[0]), (parts[0], parts[0] + 16), (b["q"], 0), (b["k"], 0), (0, b["gq"]), (b["gk"], 0), (0, b["dq"]), (b["dk"], 0), (b["wq"], 0), (0, b["wk"]), (at, 0)):
+        if all(x % 16 == 0 for x in a):
+            with pytest.raises(L.HipError, match="overlap"):
+                leave(*a)
+    # rows that interleave at different strides
+    with pytest.raises(L.HipError, match="overlap"):
+        fwd(rows=8, T=8, places=0, qo=b["q"] + 4 * Hq * hd, ldqo=3 * Hq * hd, ldq=2 * Hq * hd)
+    gpu.sync([])
+    assert all(np.array_equal(gpu.read_state_buffer(x, hd), before[m]) for m, x in b.items())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 6])
+def test_slices_of_one_product_and_rows_in_place(gpu, bufs, hd):  # noqa: F811
+    """q and k, their rotated rows, gradients and results each as slices of one wider row; over their inputs; one row, whose stride is of no account."""
+    L = mod("lib")
+    for rows, Hq, Hkv in ((13, 4, 2), (1, 4, 2)):
+        q, k, wq, wk, gq, gk = inputs(rows, Hq, Hkv, hd, 63)
+        ld, step = (Hq + Hkv) * hd + 4, 4 * Hq * hd
+        pair = lambda a, b_: np.concatenate([a.reshape(rows, -1), b_.reshape(rows, -1), np.full((rows, 4), 7.0, np.float32)], axis=1).astype(np.float32)  # noqa: E731
+        x, g, o, d = (bufs.put(a) for a in (pair(q, k), pair(gq, gk), pair(0 * q, 0 * k), pair(0 * q, 0 * k)))
+        bwq, bwk, dwq, dwk = (bufs.put(a) for a in (wq, wk, wq, wk))
+        cs = angles(rows, rows, hd, 1e4, 0)
+        wants = [ref_fwd(a, w, cs) for a, w in ((q, wq), (k, wk))]
+        grads = [ref_bwd(a, w, h, cs, True) for a, w, h in ((q, wq, gq), (k, wk, gk))]
+
+        def read(buf):
+            a = gpu.read_state_buffer(buf, rows * ld).reshape(rows, ld)
+            assert np.all(a[:, -4:] == 7.0)
+            return a[:, :Hq * hd].reshape(q.shape), a[:, Hq * hd:-4].reshape(k.shape)
+
+        def check_fwd(buf):
+            for got, (want, size) in zip(read(buf), wants):
+                assert np.all(np.abs(got - want) <= 24 * U * size)
+
+        def check_bwd(buf):
+            for got, (dx, dw, off, offw), b_ in zip(read(buf), grads, (dwq, dwk)):
+                assert np.all(np.abs(got - dx) <= off + 2 * U * np.abs(dx))
+                assert np.all(np.abs(gpu.read_state_buffer(b_, hd) - dw) <= offw + 2 * U * np.abs(dw))
+
+        def fwd(out):
+            a = forward_args(rows, Hq, Hkv, hd, q=x, ldq=ld, wq=bwq, qo=out, ldqo=ld, k=x + step, ldk=ld, wk=bwk, ko=out + step, ldko=ld)
+            L.check(gpu.ctx, L.lib.gt_qk_norm_rope_fwd(gpu.ctx, *a.values()), "fwd")
+
+        def bwd(out, up):
+            a = backward_args(rows, Hq, Hkv, hd, q=x, ldq=ld, wq=bwq, gq=up, ldgq=ld, dq=out, dwq=dwq, k=x + step, ldk=ld, wk=bwk, gk=up + step, ldgk=ld, dk=out + step, dwk=dwk)
+            L.check(gpu.ctx, L.lib.gt_qk_norm_rope_bwd(gpu.ctx, *a.values()), "bwd")
+        fwd(o)
+        check_fwd(o)
+        bwd(d, g)
+        check_bwd(d)
+        over = bufs.put(pair(gq, gk))
+        bwd(over, over)                                  # over the gradients
+        check_bwd(over)
+        bwd(x, g)                                        # over the rows themselves
+        check_bwd(x)
+        gpu.write_state_buffer(x, pair(q, k))
+        fwd(x)
+        check_fwd(x)
