@@ -356,7 +356,7 @@ static int qk_bwd_groups(gt_ctx *ctx, int64_t rows, int heads, int hd) {
 
 static int qk_check(gt_ctx *ctx, const char *who, int rows, int T, int Hq, int Hkv, int hd, double base, gt_buf places, gt_buf q, int64_t ldq,
                     gt_buf wq, gt_buf k, int64_t ldk, gt_buf wk, int64_t ldqo, int64_t ldko) {
-  GT_REQUIRE(ctx, rows >= 0 && T >= 1 && Hq >= 1 && Hkv >= 1 && q && wq && k && wk, "%s: bad arguments (rows %d, T %d, heads %d and %d)", who, rows,
+  GT_REQUIRE(ctx, rows >= 0 && (T >= 1 || places) && Hq >= 1 && Hkv >= 1 && q && wq && k && wk, "%s: bad arguments (rows %d, T %d, heads %d and %d)", who, rows,
              T, Hq, Hkv);
   GT_REQUIRE(ctx, hd >= 2 && hd % 2 == 0 && hd <= QK_MAX_HD, "%s: head size %d is not an even number up to %d", who, hd, QK_MAX_HD);
   GT_REQUIRE(ctx, base > 0 && base <= 1.7976931348623157e308, "%s: the rotation's base must be positive and finite", who);

@@ -191,3 +191,23 @@ def test_slices_of_one_product_and_rows_in_place(gpu, bufs, hd):  # noqa: F811
         gpu.write_state_buffer(x, pair(q, k))
         fwd(x)
         check_fwd(x)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [0, -3])
+def test_with_positions_the_sequence_length_is_not_read(gpu, bufs, T):  # noqa: F811
+    L = mod("lib")
+    rows, hd = 5, 64
+    q, k, wq, wk, gq, gk = inputs(rows, 2, 1, hd, 64)
+    at = [3, 0, 70000, 3, 12]
+    b = dict(q=bufs.put(q), k=bufs.put(k), wq=bufs.put(wq), wk=bufs.put(wk), places=bufs.put(np.array(at, np.int32)))
+    o, d = [bufs.raw(a.nbytes) for a in (q, k)], [bufs.raw(a.nbytes) for a in (q, k, wq, wk)]
+    L.check(gpu.ctx, L.lib.gt_qk_norm_rope_fwd(gpu.ctx, *forward_args(rows, 2, 1, hd, **{**b, "T": T}, qo=o[0], ko=o[1]).values()), "fwd")
+    L.check(gpu.ctx, L.lib.gt_qk_norm_rope_bwd(gpu.ctx, *backward_args(rows, 2, 1, hd, **{**b, "T": T}, gq=bufs.put(gq), gk=bufs.put(gk), dq=d[0], dk=d[1], dwq=d[2], dwk=d[3]).values()), "bwd")
+    cs = angles(rows, 1, hd, 1e4, 0, at)
+    for x, w, g, out, dx_, dw_ in ((q, wq, gq, o[0], d[0], d[2]), (k, wk, gk, o[1], d[1], d[3])):
+        want, size = ref_fwd(x, w, cs)
+        dx, dw, off, offw = ref_bwd(x, w, g, cs, True)
+        assert np.all(np.abs(gpu.read_state_buffer(out, x.size).reshape(x.shape) - want) <= 24 * U * size)
+        assert np.all(np.abs(gpu.read_state_buffer(dx_, x.size).reshape(x.shape) - dx) <= off + 2 * U * np.abs(dx))
+        assert np.all(np.abs(gpu.read_state_buffer(dw_, hd) - dw) <= offw + 2 * U * np.abs(dw))
