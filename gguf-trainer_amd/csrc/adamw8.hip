@@ -94,12 +94,26 @@ __device__ __forceinline__ unsigned wave_umax(unsigned v) {
   return max(max(a, b), max(c, d));
 }
 
-// sqrt(v) to the last bit or next to it: the hardware's 1 / sqrt and one Newton step. Zero stays zero, infinity and NaN give NaN; below
-// 2^-126 the result is small, but not zero.
+// sqrt(v) to the last bit or next to it: the hardware's 1 / sqrt, which takes no denormals, and one Newton step. Zero stays zero, infinity and
+// NaN give NaN.
 __device__ __forceinline__ float root(float v) {
   const float y = __builtin_amdgcn_rsqf(__builtin_amdgcn_fmed3f(v, 1.17549435e-38f, __builtin_inff()));
   const float s = v * y;
   return __builtin_fmaf(__builtin_fmaf(-s, s, v), 0.5f * y, s);
+}
+// Of four. Denormals are rare (a block that has had no gradient for a thousand steps), so they are looked for together and taken as 2^64 v.
+__device__ __forceinline__ void roots(const float (&v)[4], float (&r)[4]) {
+  unsigned least = ~0u;
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    r[j] = root(v[j]);
+    least = min(least, __float_as_uint(v[j]) - 1u);            // zero is the largest here
+  }
+  if (least < 0x7fffffu) {
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      if (v[j] < 1.17549435e-38f) r[j] = root(v[j] * 1.84467441e19f) * 2.32830644e-10f;
+  }
 }
 
 #define FINITE_BITS 0x7f800000u                  // bits of a finite magnitude are below this
@@ -233,7 +247,10 @@ __global__ __launch_bounds__(256) void adamw8_update_k(const Chunk8 *__restrict_
     const float x = gg[j] * sc;
     m[j] = m[j] * h.b1 + x * h.omb1;
     v[j] = (v[j] * v[j]) * h.b2 + (x * h.omb2) * x;
-    r[j] = root(v[j]);
+  }
+  roots(v, r);
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
     // 1 / x to the last bit but one: the update is a small part of the weight
     float upd = (m[j] * h.ibc1) * __builtin_amdgcn_rcpf(__builtin_fmaf(r[j], h.rbc2, h.eps));
     if (h.wd > 0.f) upd = __builtin_fmaf(h.wd, ww[j], upd);
@@ -309,8 +326,7 @@ __global__ __launch_bounds__(256) void state8_write_k(int64_t size, unsigned cha
     const unsigned half[4] = {0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
 #pragma unroll
     for (int j = 0; j < 4; j++) if (i0 + j < n) { mm[j] = m[b * BLK8 + i0 + j]; vv[j] = v[b * BLK8 + i0 + j] + 0.f; }      // -0 becomes 0
-#pragma unroll
-    for (int j = 0; j < 4; j++) rr[j] = root(vv[j]);
+    roots(vv, rr);
     unsigned mc, rc;
     int em, er;
     encode_block(mm, vv, rr, half, mc, rc, em, er);

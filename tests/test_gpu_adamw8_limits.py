@@ -1,0 +1,114 @@
+"""AdamW with 8-bit moments where FP32 ends: second moments that are denormal, vanish or overflow; what is read, written and read again; buffers
+that may not share memory. The states are held to the definition of test_gpu_adamw8.py, formed here from the second moments as FP32 holds them."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from gpu_common import mod
+from test_gpu_adamw8 import B1, BLK, E4M3, NEAR, Group, U, blocks_of, decode, random_words
+
+F = np.float32
+
+
+class Moments:
+    """Read and write access to tensor i of a group."""
+
+    def __init__(self, gpu, G, i=0):
+        self.gpu, self.G, self.i, self.n = gpu, G, i, G.sizes[i]
+        self.b = [gpu.create_state_buffer(4 * self.n) for _ in range(2)]
+
+    def read(self):
+        self.G.check(self.G.L.lib.gt_adamw8_read(self.gpu.ctx, self.G.h, self.i, *self.b))
+        return tuple(self.gpu.read_state_buffer(b, self.n) for b in self.b)
+
+    def write(self, m, v):
+        for b, a in zip(self.b, (m, v)):
+            self.gpu.write_state_buffer(b, np.asarray(a, F))
+        self.G.check(self.G.L.lib.gt_adamw8_write(self.gpu.ctx, self.G.h, self.i, *self.b))
+
+    def free(self):
+        for b in self.b:
+            self.gpu.free_state_buffer(b)
+
+
+def same(a, b):
+    return all(np.array_equal(x, y, equal_nan=True) for x, y in zip(a, b))
+
+
+def check_roots(x, codes, e, bits16):
+    """Codes of the roots x at the block's exponent: no element leaves e4m3's range, no exponent is more than it takes (or than the least that is
+    held), and a code is off by a step only where what is rounded lies within NEAR of a whole number of steps."""
+    top = blocks_of(x).max(axis=1)
+    with np.errstate(divide="ignore"):
+        need = np.where(top > 0, np.ceil(np.log2(top / 448)), -126).clip(-126)
+    assert np.all(e >= need) and np.all(e <= np.maximum(need, -65)), (e, need)
+    y = x / 2.0 ** np.repeat(e.astype(np.float64), BLK)[:x.size]
+    step = 2.0 ** (np.floor(np.log2(np.maximum(y, 2.0 ** -6))) - 3)
+    raw = y / step + bits16 / 65536
+    low, high = (np.where(x > 0, np.maximum(np.floor(raw + d) * step, 2.0 ** -9), 0) for d in (-NEAR, NEAR))
+    got = E4M3[codes]
+    bad = (got != low) & (got != high)
+    assert not bad.any(), f"{bad.sum()} codes, first at {np.argmax(bad)}: {got[bad][0]} for {y[bad][0]} + {bits16[bad][0]}/65536"
+
+
+def roots_of(rs, powers, spread):
+    """One block for each power: values of e4m3's four bits, the largest 15/8 * 2^power, down to 2^-spread of it, some zero."""
+    out = []
+    for p in powers:
+        r = (8 + rs.randint(0, 8, BLK)) / 8 * 2.0 ** (p - rs.randint(0, spread + 1, BLK))
+        r[rs.rand(BLK) < 0.1] = 0
+        r[0] = 15 / 8 * 2.0 ** p
+        out.append(r)
+    return np.concatenate(out)
+
+
+@pytest.mark.gpu
+def test_denormal_second_moments_out_and_in_again(gpu):
+    """v from 2^-120 down to where FP32 ends. Every r here is a multiple of 2^-74 of at most four bits, so its square is an FP32 number, and v, its root
+    and its code are exact whatever is added for the rounding."""
+    rs = np.random.RandomState(71)
+    r = roots_of(rs, (-60, -61, -62, -63, -64, -65, -67, -68), 3)
+    r[-BLK:] = roots_of(rs, (-71,), 0)
+    v, m = (r * r).astype(F), (1e-9 * rs.standard_normal(r.size)).astype(F)
+    assert np.array_equal(v.astype(np.float64), r * r) and v[v > 0].min() < 2.0 ** -140
+    G = Group(gpu, [np.zeros(r.size, F)])
+    M = Moments(gpu, G)
+    try:
+        M.write(m, v)
+        first = M.read()
+        assert np.array_equal(first[1], v)
+        mc, rc, em, er = G.states(0)
+        check_roots(r, rc, er, np.full(r.size, 32768.0))
+        M.write(*first)
+        assert same(M.read(), first)
+    finally:
+        M.free()
+        G.free()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("b2", [0.95, 0.999])
+def test_a_step_on_denormal_second_moments(gpu, b2):
+    """Without a gradient a step leaves v b2, rounded to FP32 once. Its root is within 2^-22 of itself, the weight's update as the module's text in
+    test_gpu_adamw8.py derives it."""
+    rs = np.random.RandomState(72)
+    r = roots_of(rs, (-58, -60, -62, -63, -64, -65, -66, -67), 3)
+    v, m = (r * r).astype(F), (2.0 ** -70 * rs.standard_normal(r.size)).astype(F)
+    w = (2.0 ** -12 * rs.standard_normal(r.size)).astype(F)
+    G = Group(gpu, [w], clip=0.0, wd=0.0, b2=b2)
+    M = Moments(gpu, G)
+    try:
+        M.write(m, v)
+        m0 = decode(*(lambda s: (s[0], s[2]))(G.states(0)))
+        G.step(5, lr=1e-3, seed=99)
+        want = ((r * r).astype(F) * F(b2)).astype(F).astype(np.float64)
+        words = random_words(99, 0, r.size)
+        mc, rc, em, er = G.states(0)
+        check_roots(np.sqrt(want), rc, er, (words >> np.uint64(16)).astype(np.float64))
+        m1 = B1 * m0
+        upd = 1e-3 * m1 / (1 - B1 ** 5) / (np.sqrt(want / (1 - b2 ** 5)) + 1e-8)
+        assert np.all(np.abs(G.weights(0) - (w - upd)) <= 16 * U * np.abs(upd) + 2 * U * (np.abs(w) + np.abs(w - upd)))
+    finally:
+        M.free()
+        G.free()
