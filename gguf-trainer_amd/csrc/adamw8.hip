@@ -12,7 +12,7 @@
 // two-thousandth (b2 = 0.999) of what separates it from its target, far less than half of e4m3's steps of 6 to 12 percent:
 // rounded to nearest both would stay where they are. The random bits of an element are a function of the step's seed, the
 // number of its block in the group and its place in the block, 16 for each moment, so a step repeats bit for bit. An r that
-// is there is never rounded to zero: m / (0 + eps) would follow. r is unbiased, so v = r^2 is high by r's variance: where v still
+// is there is not rounded to zero: m / (0 + eps) would follow. r is unbiased, so v = r^2 is high by r's variance: where v still
 // grows by small steps up to 6 percent, half of that in the update's denominator.
 // The update itself uses m and v before they are rounded. A moment that is not finite is held as e4m3's NaN (its weight is
 // not finite either) and its neighbours' exponent goes by the finite ones.
@@ -70,12 +70,14 @@ __device__ __forceinline__ int exponent_m(unsigned top) {
   normal_bits(top, e, frac);
   return top ? max(e - 127 - (frac <= 0x600000u ? 8 : 7), -126) : -126;
 }
-// the same for sqrt(top): top <= 448^2 * 4^e, 448^2 = 1.53125 * 2^17
+// the same for sqrt(top), e >= LEAST_R: top <= 448^2 * 4^e, 448^2 = 1.53125 * 2^17. With it every r is a multiple of 2^-74 of at most four bits,
+// and its square an FP32 number: none is lost where the step forms it or in FP32 moments, though it were the last of the denormals.
+#define LEAST_R -65
 __device__ __forceinline__ int exponent_r(unsigned top) {
   int e;
   unsigned frac;
   normal_bits(top, e, frac);
-  return top ? (e - 127 - (frac <= 0x440000u ? 17 : 16) + 1) >> 1 : -126;
+  return top ? max((e - 127 - (frac <= 0x440000u ? 17 : 16) + 1) >> 1, LEAST_R) : -126;
 }
 
 // Largest of one word over the wavefront, as a scalar: four exchanges within each row of 16 lanes, the four rows on the

@@ -334,7 +334,7 @@ int gt_adamw_destroy(gt_ctx *ctx, gt_adamw *opt);
 /* The same step with the moments held in 8 bits: 2 bytes of state per parameter instead of 8, 16 (20 with the clip) bytes moved per
  * parameter and step instead of 28 (32). No counterpart in the reference. m[i] and r[i] are sizes[i] bytes each: the first moment
  * and the ROOT of the second as OCP e4m3 values; e[i] holds two signed bytes for each block of 256 elements (2 * ceil(sizes[i] / 256)
- * bytes, 2-byte aligned), the exponents of m and of r: a state is its e4m3 value times 2^e. All bytes zero = zero moments. The
+ * bytes, 2-byte aligned), the exponents of m (-126 or more) and of r (-65 or more; -126 in a block of zeros): a state is its e4m3 value times 2^e. All bytes zero = zero moments. The
  * caller owns and clears the buffers. Each step rounds the new moments up or down at random in proportion, from bits that `seed`,
  * the block and the place in it determine: pass another seed each step (the step number will do); the same seed gives the
  * same bits. Gradients and weights are FP32, the update uses the moments before they are rounded, and the norm for the

@@ -112,3 +112,36 @@ def test_a_step_on_denormal_second_moments(gpu, b2):
     finally:
         M.free()
         G.free()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("b2", [0.5, 0.95])
+def test_second_moments_that_decay_for_good(gpu, b2):
+    """Blocks that get no gradient any more (embedding rows that no batch names). Their second moments stop at 2^-148, the square of the least root that
+    is held: one that is there stays there, and at every step read and write give back what was held and a run that goes through them
+    does what one without them does."""
+    rs = np.random.RandomState(73)
+    r = roots_of(rs, (-55, -58, -62, -66), 3)
+    v, m = (r * r).astype(F), (2.0 ** -70 * rs.standard_normal(r.size)).astype(F)
+    G = [Group(gpu, [np.zeros(r.size, F)], clip=0.0, wd=0.0, b2=b2) for _ in range(2)]
+    M = [Moments(gpu, g) for g in G]
+    try:
+        for x in M:
+            x.write(m, v)
+        floors = 0
+        for t in range(1, 61 if b2 < 0.9 else 501):
+            for g in G:
+                g.step(t)
+            if t % 20 and t < 40:
+                continue
+            held = M[1].read()
+            M[1].write(*held)
+            again = M[1].read()
+            assert same(held, again) and same(held, M[0].read()), t
+            assert np.array_equal(held[1] > 0, r > 0), t
+            floors += np.all(held[1][r > 0] < 2.0 ** -140)
+        assert floors > 0                                                    # they got there
+        assert np.array_equal(G[0].weights(0), G[1].weights(0))
+    finally:
+        for x in M + G:
+            x.free()
