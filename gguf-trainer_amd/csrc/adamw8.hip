@@ -14,8 +14,9 @@
 // number of its block in the group and its place in the block, 16 for each moment, so a step repeats bit for bit. An r that
 // is there is not rounded to zero: m / (0 + eps) would follow. r is unbiased, so v = r^2 is high by r's variance: where v still
 // grows by small steps up to 6 percent, half of that in the update's denominator.
-// The update itself uses m and v before they are rounded. A moment that is not finite is held as e4m3's NaN (its weight is
-// not finite either) and its neighbours' exponent goes by the finite ones.
+// The update itself uses m and v before they are rounded. Moments that are not finite are held as e4m3's NaN, and their neighbours'
+// exponent goes by the finite ones. r has no use for the sign: its positive NaN stands for infinity, a square that left FP32, whose weight is
+// left to its decay as with moments of 32 bits, its negative one for NaN.
 //
 // Bound by memory: 16 bytes per element (g read, w read and written, two codes each way), 20 with the clip, whose norm has
 // to be known before the first update. One wavefront to a block, four neighbouring elements to a lane, so that the block's
@@ -96,6 +97,8 @@ __device__ __forceinline__ unsigned wave_umax(unsigned v) {
   return max(max(a, b), max(c, d));
 }
 
+#define FINITE_BITS 0x7f800000u                  // bits of a finite magnitude are below this
+
 // sqrt(v) to the last bit or next to it: the hardware's 1 / sqrt, which takes no denormals, and one Newton step. Zero stays zero, infinity and
 // NaN give NaN.
 __device__ __forceinline__ float root(float v) {
@@ -103,22 +106,24 @@ __device__ __forceinline__ float root(float v) {
   const float s = v * y;
   return __builtin_fmaf(__builtin_fmaf(-s, s, v), 0.5f * y, s);
 }
-// Of four. Denormals are rare (a block that has had no gradient for a thousand steps), so they are looked for together and taken as 2^64 v.
+// Of four. Denormals (a block that has had no gradient for a thousand steps) and infinity are rare, so they are looked for together: the former
+// are taken as 2^64 v, the latter stays itself.
 __device__ __forceinline__ void roots(const float (&v)[4], float (&r)[4]) {
-  unsigned least = ~0u;
+  unsigned least = ~0u, most = 0;
 #pragma unroll
   for (int j = 0; j < 4; j++) {
     r[j] = root(v[j]);
     least = min(least, __float_as_uint(v[j]) - 1u);            // zero is the largest here
+    most = max(most, __float_as_uint(v[j]));
   }
-  if (least < 0x7fffffu) {
+  if (least < 0x7fffffu || most >= FINITE_BITS) {
 #pragma unroll
-    for (int j = 0; j < 4; j++)
+    for (int j = 0; j < 4; j++) {
       if (v[j] < 1.17549435e-38f) r[j] = root(v[j] * 1.84467441e19f) * 2.32830644e-10f;
+      if (__float_as_uint(v[j]) == FINITE_BITS) r[j] = v[j];
+    }
   }
 }
-
-#define FINITE_BITS 0x7f800000u                  // bits of a finite magnitude are below this
 
 // Four codes, one to a byte, from the magnitudes of four values scaled so that e4m3's exponent is theirs: y = |value| * 2^(-e - 120). A y
 // below 2^-126 is then a denormal exactly where e4m3's are, so one addition rounds both: the code is the y's bits from 20
@@ -134,6 +139,9 @@ __device__ __forceinline__ unsigned gather(const unsigned (&t)[4]) {
   return lo | hi;
 }
 
+#define INF_R 0x7fu                              // codes of an r that is infinite
+#define NAN_R 0xffu                              // and of one that is no number
+
 // Codes and exponents of a block's moments from their values and roots, four elements to a lane (elements past the tensor's
 // end as zeros). bits: 16 random bits for m below 16 for r.
 __device__ __forceinline__ void encode_block(const float (&m)[4], const float (&v)[4], const float (&r)[4], const unsigned (&bits)[4], unsigned &mc,
@@ -144,7 +152,8 @@ __device__ __forceinline__ void encode_block(const float (&m)[4], const float (&
   for (int j = 0; j < 4; j++) { am[j] = __float_as_uint(m[j]) & 0x7fffffffu; av[j] = __float_as_uint(v[j]); }
   unsigned tm = wave_umax(max(max(am[0], am[1]), max(am[2], am[3])));
   unsigned tv = wave_umax(max(max(av[0], av[1]), max(av[2], av[3])));
-  if (max(tm, tv) >= FINITE_BITS) {              // an infinity, a NaN, a second moment below zero: the exponents go by the others
+  const bool odd = max(tm, tv) >= FINITE_BITS;
+  if (odd) {                                     // an infinity, a NaN, a second moment below zero: the exponents go by the others
     tm = tv = 0;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -165,10 +174,21 @@ __device__ __forceinline__ void encode_block(const float (&m)[4], const float (&
   }
   mc = gather(cm);
   rc = gather(cr);
+  if (odd) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) if (!(v[j] >= 0.f)) rc |= NAN_R << (8 * j);
+  }
 }
 __device__ __forceinline__ void decode4(unsigned c, float s, float (&out)[4]) {
   const v2f lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, true);
   out[0] = lo[0] * s; out[1] = lo[1] * s; out[2] = hi[0] * s; out[3] = hi[1] * s;
+}
+__device__ __forceinline__ void decode_roots4(unsigned c, float s, float (&out)[4]) {
+  decode4(c, s, out);
+  if (((c & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) {       // a NaN among them
+#pragma unroll
+    for (int j = 0; j < 4; j++) if ((c >> (8 * j) & 0xffu) == INF_R) out[j] = __builtin_inff();
+  }
 }
 // four neighbouring bytes of a block of n elements; zeros past its end
 __device__ __forceinline__ unsigned load_codes(const gbyte *p, int i0, int n, bool whole) {
@@ -241,7 +261,7 @@ __global__ __launch_bounds__(256) void adamw8_update_k(const Chunk8 *__restrict_
     for (int j = 0; j < 4; j++) if (i0 + j < n) { gg[j] = g[i0 + j]; ww[j] = w[i0 + j]; }
   }
   decode4(load_codes(mp, i0, n, whole), pow2(e[0]), m);
-  decode4(load_codes(rp, i0, n, whole), pow2(e[1]), v);
+  decode_roots4(load_codes(rp, i0, n, whole), pow2(e[1]), v);
   const unsigned key = mix2((c.block + b) ^ h.key) + (unsigned)i0 * 0x9E3779B9u;
   unsigned bits[4];
 #pragma unroll
@@ -315,7 +335,7 @@ __global__ __launch_bounds__(256) void state8_read_k(int64_t size, const unsigne
     if (m) m[i] = __builtin_amdgcn_cvt_f32_fp8((int)mp[i], 0) * pow2(e[2 * b]);
     if (v) {
       const float r = __builtin_amdgcn_cvt_f32_fp8((int)rp[i], 0) * pow2(e[2 * b + 1]);
-      v[i] = r * r;
+      v[i] = rp[i] == INF_R ? __builtin_inff() : r * r;
     }
   }
 }

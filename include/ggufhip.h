@@ -338,7 +338,9 @@ int gt_adamw_destroy(gt_ctx *ctx, gt_adamw *opt);
  * caller owns and clears the buffers. Each step rounds the new moments up or down at random in proportion, from bits that `seed`,
  * the block and the place in it determine: pass another seed each step (the step number will do); the same seed gives the
  * same bits. Gradients and weights are FP32, the update uses the moments before they are rounded, and the norm for the
- * clip is summed in 64 bits. A moment that is not finite is held as NaN. The handle is gt_adamw's: gt_adamw_grad_norm and
+ * clip is summed in 64 bits. A moment that is not finite is held as e4m3's NaN; of r
+ * the positive one stands for infinity (a square that left FP32: its weight is left to its decay, as by gt_adamw_step), the negative one
+ * for NaN. The handle is gt_adamw's: gt_adamw_grad_norm and
  * gt_adamw_destroy take it, gt_adamw_step does not. A step allocates nothing. No two of the w, m, r and e buffers may overlap.
  *   gt_adamw8_read:  the moments of tensor i as FP32 values, m and v = r^2 (0: not wanted)
  *   gt_adamw8_write: the states of tensor i from FP32 moments, rounded to nearest; what gt_adamw8_read gave comes back unchanged */

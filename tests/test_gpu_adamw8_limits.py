@@ -145,3 +145,91 @@ def test_second_moments_that_decay_for_good(gpu, b2):
     finally:
         for x in M + G:
             x.free()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("wd", [0.0, 0.1])
+def test_second_moments_that_overflow(gpu, wd):
+    """A gradient whose square leaves FP32 while the first moment does not: the weight is left to its decay, in this step and in all later ones, as it is
+    with moments of 32 bits (m / infinity). The block's other elements are stepped as without it, and the moments come back as infinities."""
+    n, at, t0 = 3 * BLK + 5, (7, 2 * BLK + 1, 3 * BLK + 4), 1
+    rs = np.random.RandomState(74)
+    w, g = rs.standard_normal(n).astype(F), rs.standard_normal(n).astype(F)
+    big = g.copy()
+    for i, x in zip(at, (6e20, -1e30, 3e38)):
+        big[i] = x
+    zero = g.copy()
+    zero[list(at)] = 0
+    G = Group(gpu, [w], clip=0.0, wd=wd)
+    H = Group(gpu, [w], clip=0.0, wd=wd)
+    M = Moments(gpu, G)
+    L = mod("lib")
+    b32 = [gpu.create_state_buffer(4 * n) for _ in range(4)]
+    h32 = C.c_void_p()
+    one = lambda b: (L.buf * 1)(b)  # noqa: E731
+    L.check(gpu.ctx, L.lib.gt_adamw_create(gpu.ctx, 1, *[one(b) for b in b32], (C.c_int64 * 1)(n), B1, 0.999, 1e-8, wd, 0.0, C.byref(h32)), "create")
+    gpu.write_state_buffer(b32[0], w)
+    try:
+        other = np.ones(n, bool)
+        other[list(at)] = False
+        for t, (a, b) in enumerate(((big, zero), (g, zero), (zero, zero), (g, zero)), t0):
+            G.grads([a])
+            H.grads([b])
+            gpu.write_state_buffer(b32[1], a)
+            for x in (G, H):
+                x.step(t)
+            L.check(gpu.ctx, L.lib.gt_adamw_step(gpu.ctx, h32, 1e-3, 1 - B1 ** t, 1 - 0.999 ** t), "step")
+            got, alone, full = G.weights(0), H.weights(0), gpu.read_state_buffer(b32[0], n)
+            # both sides round the decay three times, lr, wd and the product with w, and the weight once
+            assert np.all(np.abs(got[list(at)] - full[list(at)]) <= t * (8 * U * 1e-3 * wd + 2 * U) * np.abs(w[list(at)])), (got[list(at)], full[list(at)])
+            if t == 1:
+                assert np.array_equal(got[other], alone[other])              # the update does not depend on what the block's exponent rounds
+            m, v = M.read()
+            assert np.all(np.isposinf(v[list(at)])) and np.all(np.isfinite(v[other])) and np.all(np.isfinite(m)) and np.all(np.isfinite(got))
+            M.write(m, v)
+            assert same(M.read(), (m, v))
+    finally:
+        L.check(gpu.ctx, L.lib.gt_adamw_destroy(gpu.ctx, h32), "destroy")
+        for b in b32:
+            gpu.free_state_buffer(b)
+        M.free()
+        G.free()
+        H.free()
+
+
+@pytest.mark.gpu
+def test_moments_that_are_no_numbers(gpu):
+    """A first moment that is infinite or NaN takes its weight with it, as in 32 bits. A second moment that is NaN or negative comes back as NaN, takes its
+    weight with it and stays; none of them touches a neighbour."""
+    n = 2 * BLK + 9
+    rs = np.random.RandomState(75)
+    w, g = rs.standard_normal(n).astype(F), rs.standard_normal(n).astype(F)
+    m, v = rs.standard_normal(n).astype(F), (rs.standard_normal(n) ** 2).astype(F)
+    bad_m, bad_v = {3: np.inf, BLK + 9: np.nan, 2 * BLK + 8: -np.inf}, {5: np.nan, BLK + 1: -1.0, 2 * BLK: -np.inf, BLK + 77: -1e-42}
+    inf_v = {8: np.inf, 2 * BLK + 3: np.inf}
+    G, H = Group(gpu, [w], clip=0.0, wd=0.1), Group(gpu, [w], clip=0.0, wd=0.1)
+    M, K = Moments(gpu, G), Moments(gpu, H)
+    try:
+        mm, vv = m.copy(), v.copy()
+        for d, a, z in ((bad_m, mm, m), (bad_v, vv, v), (inf_v, vv, v)):
+            for i, x in d.items():
+                a[i], z[i] = x, 0
+        M.write(mm, vv)
+        K.write(m, v)
+        fine = np.ones(n, bool)
+        fine[[*bad_m, *bad_v, *inf_v]] = False
+        for t in (3, 4):
+            a, b = M.read(), K.read()
+            assert all(np.array_equal(x[fine], y[fine]) for x, y in zip(a, b))
+            assert np.all(np.isnan(a[0][list(bad_m)])) and np.all(np.isnan(a[1][list(bad_v)])) and np.all(np.isposinf(a[1][list(inf_v)]))
+            M.write(*a)
+            assert same(M.read(), a)
+            for x in (G, H):
+                x.grads([g])
+                x.step(t)
+            ga, gb = G.weights(0), H.weights(0)
+            assert np.array_equal(ga[fine], gb[fine])
+            assert np.all(np.isnan(ga[[*bad_m, *bad_v]])) and np.all(np.isfinite(ga[list(inf_v)]))
+    finally:
+        for x in (M, K, G, H):
+            x.free()
