@@ -139,6 +139,12 @@ __device__ __forceinline__ unsigned gather(const unsigned (&t)[4]) {
   return lo | hi;
 }
 
+__device__ __forceinline__ unsigned without_256(unsigned c) {
+#pragma unroll
+  for (int j = 0; j < 4; j++) if ((c >> (8 * j) & 0x7fu) == 0x78u) c -= 1u << (8 * j);
+  return c;
+}
+
 #define INF_R 0x7fu                              // codes of an r that is infinite
 #define NAN_R 0xffu                              // and of one that is no number
 
@@ -178,6 +184,9 @@ __device__ __forceinline__ void encode_block(const float (&m)[4], const float (&
 #pragma unroll
     for (int j = 0; j < 4; j++) if (!(v[j] >= 0.f)) rc |= NAN_R << (8 * j);
   }
+  // next to FP32's largest, 256 * 2^120 is past it as an m, and the square of 256 * 2^56 as an r: 240 of them are the most that is held
+  if (em >= 120) mc = without_256(mc);
+  if (er >= 56) rc = without_256(rc);
 }
 __device__ __forceinline__ void decode4(unsigned c, float s, float (&out)[4]) {
   const v2f lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, true);

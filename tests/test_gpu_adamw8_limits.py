@@ -233,3 +233,59 @@ def test_moments_that_are_no_numbers(gpu):
     finally:
         for x in (M, K, G, H):
             x.free()
+
+
+@pytest.mark.gpu
+def test_the_largest_second_moments_stay_finite(gpu):
+    """Up to FP32's largest number: a root that is rounded up has a square that is still finite, in a step, when written and when read again."""
+    n = 4 * BLK
+    rs = np.random.RandomState(76)
+    v = (np.float64(np.finfo(F).max) * np.exp(-0.3 * rs.rand(n))).astype(F)
+    v[:4] = np.finfo(F).max, F(2.9907e38), F(3.1e38), F(3.2e38)
+    G = Group(gpu, [np.ones(n, F)], clip=0.0, wd=0.0)
+    M = Moments(gpu, G)
+    try:
+        M.write(np.ones(n), v)
+        for t in range(5, 25):
+            m, got = M.read()
+            assert np.all(np.isfinite(got)) and got.max() > 2.9e38, t
+            M.write(m, got)
+            assert same(M.read(), (m, got))
+            g = np.where(rs.rand(n) < 0.5, 5.8e20, 5.5e20).astype(F)    # with (1 - b2) g^2 finite the sum with b2 v is past FP32 or just not
+            M.write(m, np.minimum(got, F(2.9e38)) * F(0.02))
+            _, old = M.read()
+            G.grads([g])
+            G.step(t)
+            with np.errstate(over="ignore"):
+                want = old * F(0.999) + (g * F(1 - 0.999)) * g
+            _, got = M.read()
+            assert np.array_equal(np.isfinite(got), np.isfinite(want)) and np.any(np.isfinite(want) & (want > 2.9908e38)), t
+            assert np.all(np.isfinite(G.weights(0)))
+            M.write(m, v)
+    finally:
+        M.free()
+        G.free()
+
+
+@pytest.mark.gpu
+def test_the_largest_first_moments_stay_finite(gpu):
+    n = 2 * BLK
+    rs = np.random.RandomState(77)
+    m = (np.float64(np.finfo(F).max) * np.exp(-0.3 * rs.rand(n)) * np.sign(rs.standard_normal(n))).astype(F)
+    m[:4] = np.finfo(F).max, -np.finfo(F).max, F(3.2e38), F(-3.3e38)
+    G = Group(gpu, [np.ones(n, F)], clip=0.0, wd=0.0)
+    M = Moments(gpu, G)
+    try:
+        for t in range(30, 50):
+            M.write(m, np.full(n, F(1e38)))
+            got = M.read()
+            assert np.all(np.isfinite(got[0])) and np.all(np.sign(got[0]) == np.sign(m)) and np.abs(got[0]).max() > 3.1e38, t
+            M.write(*got)
+            assert same(M.read(), got)
+            G.grads([(m / 2).astype(F)])                                # its square is past FP32: v is infinite, m is not
+            G.step(t)
+            assert np.all(np.isfinite(M.read()[0])) and np.all(np.isfinite(G.weights(0))), t
+            G.gpu.write_state_buffer(G.w[0], np.ones(n, F))
+    finally:
+        M.free()
+        G.free()
