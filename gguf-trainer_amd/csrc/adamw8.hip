@@ -24,6 +24,7 @@
 // twice that (library roots and divisions, float comparisons for the block's largest) they were as long as the memory's time.
 #include <algorithm>
 #include <exception>
+#include <iterator>
 #include <utility>
 #include "optim.h"
 
@@ -407,6 +408,15 @@ int gt_adamw8_create(gt_ctx *ctx, int n, const gt_buf *w, const gt_buf *g, const
       delete o;
       GT_FAIL(ctx, "gt_adamw8_create: two of the buffers that a step writes overlap (a tensor listed twice?)");
     }
+  // and a gradient in what a step writes would be read by some workgroups before and by others after
+  for (int i = 0; i < n; i++)
+    if (sizes[i]) {
+      const auto at = std::upper_bound(spans.begin(), spans.end(), std::make_pair(g[i], UINT64_MAX));
+      if ((at != spans.begin() && std::prev(at)->second > g[i]) || (at != spans.end() && at->first < g[i] + (uint64_t)sizes[i] * 4)) {
+        delete o;
+        GT_FAIL(ctx, "gt_adamw8_create: the gradient of tensor %d and a buffer that a step writes overlap", i);
+      }
+    }
   o->bits8 = true;
   o->n = n; o->beta1 = beta1; o->beta2 = beta2; o->eps = eps; o->wd = weight_decay; o->clip = clip;
   unsigned block = 0;
@@ -481,12 +491,23 @@ static int state8_of(gt_ctx *ctx, const char *who, gt_adamw *o, int i, const Ten
   return 0;
 }
 
+static bool meet(gt_buf a, uint64_t na, const void *b, uint64_t nb) {
+  const uint64_t at = reinterpret_cast<uint64_t>(b);
+  return a && at && a < at + nb && at < a + na;
+}
+static bool meets_state(gt_buf a, const Tensor8 *t) {
+  const uint64_t n = (uint64_t)t->size, na = n * 4;
+  return meet(a, na, t->m, n) || meet(a, na, t->r, n) || meet(a, na, t->e, (uint64_t)cdiv(t->size, BLK8) * 2);
+}
+
 int gt_adamw8_read(gt_ctx *ctx, gt_adamw *o, int i, gt_buf m, gt_buf v) {
   GT_ENTER(ctx);
   const Tensor8 *t;
   if (state8_of(ctx, "gt_adamw8_read", o, i, &t)) return 1;
   GT_REQUIRE(ctx, (m | v) % 4 == 0, "gt_adamw8_read: a buffer is not aligned to its elements");
   if (t->size == 0 || (!m && !v)) return 0;
+  GT_REQUIRE(ctx, !meets_state(m, t) && !meets_state(v, t) && !meet(m, (uint64_t)t->size * 4, P<void>(v), (uint64_t)t->size * 4),
+             "gt_adamw8_read: the buffers overlap, each other or the tensor's states");
   const unsigned nb = (unsigned)std::min<int64_t>(cdiv(t->size, 256), (int64_t)ctx->num_cu * 16);
   hipLaunchKernelGGL(state8_read_k, dim3(nb), dim3(256), 0, ctx->stream, t->size, t->m, t->r, t->e, P<float>(m), P<float>(v));
   GT_LAUNCHED(ctx);
@@ -499,6 +520,7 @@ int gt_adamw8_write(gt_ctx *ctx, gt_adamw *o, int i, gt_buf m, gt_buf v) {
   if (state8_of(ctx, "gt_adamw8_write", o, i, &t)) return 1;
   GT_REQUIRE(ctx, m && v && (m | v) % 4 == 0, "gt_adamw8_write: a buffer is missing or not aligned to its elements");
   if (t->size == 0) return 0;
+  GT_REQUIRE(ctx, !meets_state(m, t) && !meets_state(v, t), "gt_adamw8_write: a buffer and the tensor's states overlap");
   const unsigned nb = (unsigned)std::min<int64_t>(cdiv(t->size, 4 * BLK8), (int64_t)ctx->num_cu * 16);
   hipLaunchKernelGGL(state8_write_k, dim3(nb), dim3(256), 0, ctx->stream, t->size, t->m, t->r, t->e, P<const float>(m), P<const float>(v));
   GT_LAUNCHED(ctx);

@@ -341,7 +341,8 @@ int gt_adamw_destroy(gt_ctx *ctx, gt_adamw *opt);
  * clip is summed in 64 bits. A moment that is not finite is held as e4m3's NaN; of r
  * the positive one stands for infinity (a square that left FP32: its weight is left to its decay, as by gt_adamw_step), the negative one
  * for NaN. The handle is gt_adamw's: gt_adamw_grad_norm and
- * gt_adamw_destroy take it, gt_adamw_step does not. A step allocates nothing. No two of the w, m, r and e buffers may overlap.
+ * gt_adamw_destroy take it, gt_adamw_step does not. A step allocates nothing. No two of the w, m, r and e buffers may overlap, and no
+ * gradient may overlap one of them.
  *   gt_adamw8_read:  the moments of tensor i as FP32 values, m and v = r^2 (0: not wanted)
  *   gt_adamw8_write: the states of tensor i from FP32 moments, rounded to nearest; what gt_adamw8_read gave comes back unchanged */
 int gt_adamw8_create(gt_ctx *ctx, int n, const gt_buf *w, const gt_buf *g, const gt_buf *m, const gt_buf *r, const gt_buf *e,

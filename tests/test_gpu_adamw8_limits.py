@@ -289,3 +289,35 @@ def test_the_largest_first_moments_stay_finite(gpu):
     finally:
         M.free()
         G.free()
+
+
+@pytest.mark.gpu
+def test_gradients_and_moment_buffers_that_overlap_are_refused(gpu):
+    """A step writes weights and states while other workgroups still read gradients; read and write of the moments go through all of a tensor at once."""
+    L = mod("lib")
+    lib = L.lib
+    n = 1000
+    b = {m: gpu.create_state_buffer(s) for m, s in dict(w=4 * n, g=4 * n, m=n, r=n, e=8, w2=4 * n, g2=4 * n, m2=n, r2=n, e2=8, x=4 * n, y=4 * n).items()}
+    h = C.c_void_p()
+
+    def create(**kw):
+        a = {**b, **kw}
+        t = lambda *v: (L.buf * 2)(*v)  # noqa: E731
+        L.check(gpu.ctx, lib.gt_adamw8_create(gpu.ctx, 2, t(a["w"], a["w2"]), t(a["g"], a["g2"]), t(a["m"], a["m2"]), t(a["r"], a["r2"]), t(a["e"], a["e2"]),
+                                              (C.c_int64 * 2)(n, n), B1, 0.999, 1e-8, 0.0, 0.0, C.byref(h)), "create")
+    try:
+        for kw in (dict(g=b["w"]), dict(g=b["w2"]), dict(g2=b["w"] + 4 * n - 4), dict(g=b["m"] - 4 * n + 4), dict(g2=b["r"]), dict(g=b["e2"]), dict(g2=b["e"])):
+            with pytest.raises(L.HipError, match="overlap"):
+                create(**kw)
+        create(g2=b["g"] + 8)                                             # gradients are only read: they may share memory
+        L.check(gpu.ctx, lib.gt_adamw8_step(gpu.ctx, h, 1e-3, 0.1, 0.1, 1), "step")
+        for call, args in ((lib.gt_adamw8_read, ((b["x"], b["x"]), (b["x"], b["x"] + 4 * n - 4), (b["m"] - b["m"] % 4, 0), (0, b["r"] - b["r"] % 4), (b["e"] - b["e"] % 4, b["y"]))),
+                           (lib.gt_adamw8_write, ((b["m"], b["y"]), (b["x"], b["r"]), (b["x"], b["e"])))):
+            for m, v in args:
+                assert call(gpu.ctx, h, 0, m, v) != 0 and "overlap" in lib.gt_last_error(gpu.ctx).decode(), (m, v)
+        L.check(gpu.ctx, lib.gt_adamw8_read(gpu.ctx, h, 0, b["x"], b["y"]), "read")
+        L.check(gpu.ctx, lib.gt_adamw8_write(gpu.ctx, h, 0, b["x"], b["x"]), "write")       # both only read
+        L.check(gpu.ctx, lib.gt_adamw_destroy(gpu.ctx, h), "destroy")
+    finally:
+        for x in b.values():
+            gpu.free_state_buffer(x)
