@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 from gpu_common import mod
-from test_gpu_adamw8 import B1, BLK, E4M3, NEAR, Group, U, blocks_of, decode, random_words
+from test_gpu_adamw8 import B1, BLK, E4M3, NEAR, Group, U, blocks_of, check_state, decode, random_words
 
 F = np.float32
 
@@ -321,3 +321,32 @@ def test_gradients_and_moment_buffers_that_overlap_are_refused(gpu):
     finally:
         for x in b.values():
             gpu.free_state_buffer(x)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [300, 2 * BLK + 9])
+def test_written_moments_that_are_none_leave_their_neighbours_exponent_alone(gpu, n):
+    """Second moments below zero, infinite or NaN and larger than all others in their block, first moments likewise: exponents and codes go by the rest."""
+    rs = np.random.RandomState(78)
+    m, v = (0.1 * rs.standard_normal(n)).astype(F), (rs.standard_normal(n) ** 2).astype(F)
+    G = Group(gpu, [np.zeros(n, F)])
+    M = Moments(gpu, G)
+    half = np.full(n, 32768.0)
+    try:
+        at = [1, 5, 130, n - 1]
+        vv, mm = v.copy(), m.copy()
+        vv[at] = -4e4, np.inf, np.nan, -np.inf
+        mm[[2, 6, 131, n - 2]] = np.inf, -np.inf, np.nan, np.inf
+        M.write(mm, vv)
+        mc, rc, em, er = G.states(0)
+        assert np.all(rc[at] & 0x7F == 0x7F)
+        x = np.where(np.isfinite(vv) & (vv >= 0), vv, 0).astype(np.float64)
+        rest = rc.copy()
+        rest[at] = 0
+        check_state(np.sqrt(x), rest, er, half, True, "r")
+        check_state(mm.astype(np.float64), mc, em, half, False, "m")
+        M.write(np.where(np.isfinite(mm), mm, 0), x)
+        assert all(np.array_equal(a, b) for a, b in zip(G.states(0)[2:], (em, er)))
+    finally:
+        M.free()
+        G.free()
