@@ -38,8 +38,16 @@ class AdamWHip:
         self.beta1, self.beta2, self.eps, self.weight_decay, self.clip = beta1, beta2, eps, weight_decay, clip
         self.t = 0
         self._m, self._v, self._e = [], [], []
-        w, g = [], []
-        per = 1 if state_bits == 8 else 4
+        self._h = C.c_void_p()
+        try:
+            self._create()
+        except Exception:
+            self.destroy()                  # a refused group keeps no memory
+            raise
+
+    def _create(self):
+        gpu, w, g = self.gpu, [], []
+        per = 1 if self.state_bits == 8 else 4
         for p in self.params:
             b = gpu.buffers_for(p)          # uploads host weights once; accumulator on the device
             gpu.keep_grad_on_device(p)
@@ -47,17 +55,17 @@ class AdamWHip:
             g.append(b["grad"])
             self._m.append(gpu.create_state_buffer(p.size * per))
             self._v.append(gpu.create_state_buffer(p.size * per))
-            if state_bits == 8:
+            if self.state_bits == 8:
                 self._e.append(gpu.create_state_buffer(2 * (-(-p.size // _BLOCK8))))
-        self._h = C.c_void_p()
         n = len(self.params)
         sizes = (C.c_int64 * max(1, n))(*[p.size for p in self.params])
-        if state_bits == 8:
+        options = (self.beta1, self.beta2, self.eps, self.weight_decay, self.clip)
+        if self.state_bits == 8:
             check(gpu.ctx, lib.gt_adamw8_create(gpu.ctx, n, _bufs(w), _bufs(g), _bufs(self._m), _bufs(self._v), _bufs(self._e), sizes,
-                                                beta1, beta2, eps, weight_decay, clip, C.byref(self._h)), "gt_adamw8_create")
+                                                *options, C.byref(self._h)), "gt_adamw8_create")
             return
         check(gpu.ctx, lib.gt_adamw_create(gpu.ctx, n, _bufs(w), _bufs(g), _bufs(self._m), _bufs(self._v), sizes,
-                                           beta1, beta2, eps, weight_decay, clip, C.byref(self._h)), "gt_adamw_create")
+                                           *options, C.byref(self._h)), "gt_adamw_create")
 
     def set_lr_scale(self, s: float):
         self.lr_scale = s

@@ -350,3 +350,23 @@ def test_written_moments_that_are_none_leave_their_neighbours_exponent_alone(gpu
     finally:
         M.free()
         G.free()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["adamw", "muon"])
+def test_a_refused_group_keeps_no_memory(gpu, which):
+    """A parameter listed twice has two sets of states that a step would write at once; what was made for them goes back."""
+    ag, optim, L = mod("autograd"), mod("optim"), mod("lib")
+    p = ag.Tensor(np.ones(3000, F), [3000], True)
+    gpu.buffers_for(p)
+    before = gpu.resident_bytes()
+    for _ in range(3):
+        with pytest.raises(L.HipError, match="overlap"):
+            if which == "adamw":
+                optim.AdamWHip(gpu, [p, p], lr=1e-3, state_bits=8)
+            else:
+                optim.MuonHip(gpu, [], [p, p], lr=0.01, aux={"lr": 1e-3, "state_bits": 8})
+    assert gpu.resident_bytes() == before
+    opt = optim.AdamWHip(gpu, [p], lr=1e-3, state_bits=8)
+    opt.destroy()
+    assert gpu.resident_bytes() == before
