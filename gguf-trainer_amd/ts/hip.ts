@@ -768,6 +768,13 @@ export class HipBackend implements OpsBackend, RegionBackend {
     posOffset: number,
   ): [Tensor, Tensor] {
     if (q === k || qw === kw) throw new Error("qkNormRope: q and k, and their gains, must be distinct tensors");
+    const sides: [Tensor, Tensor, number, string][] = [[q, qw, Hq, "q"], [k, kw, Hkv, "k"]];
+    for (const [t, w, H, name] of sides) {
+      if (t.shape.length !== 2 || t.shape[1] !== H * hd || prod(w.shape) !== hd) {
+        throw new Error(`qkNormRope: ${name} is [${t.shape.join(", ")}] with a gain of ${prod(w.shape)}, expected ${H} heads of ${hd}`);
+      }
+    }
+    if (q.shape[0] !== k.shape[0]) throw new Error(`qkNormRope: q has ${q.shape[0]} rows and k ${k.shape[0]}`);
     const rows = q.shape[0], ldq = BigInt(Hq * hd), ldk = BigInt(Hkv * hd);
     const qd = this.dataOf(q), kd = this.dataOf(k), qwd = this.dataOf(qw), kwd = this.dataOf(kw);
     const { t: qo, e: eq } = this.makeOut([rows, Hq * hd], [q, k, qw, kw]);

@@ -1,0 +1,98 @@
+"""What hip.ts does before and around its library calls, run: bodies of the binding are taken out of the file, their type annotations dropped, and
+executed by node against a stand-in for the library that records the calls. (Deno is not needed for that, and not here.)"""
+import json
+import os
+import re
+import shutil
+import subprocess
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+SRC = open(os.path.join(ROOT, "gguf-trainer_amd", "ts", "hip.ts")).read()
+needs_node = pytest.mark.skipif(shutil.which("node") is None, reason="no node")
+
+
+def block(src, at):
+    """The text from the first brace at or after `at` to the one that closes it."""
+    i = src.index("{", at)
+    depth, j = 0, i
+    while True:
+        depth += {"{": 1, "}": -1}.get(src[j], 0)
+        j += 1
+        if not depth:
+            return src[i:j]
+
+
+def plain(body):
+    """Without the annotations that occur in these bodies."""
+    body = re.sub(r"\bas (\[[^\]]*\]|\w+)(\[\])?", "", body)
+    body = re.sub(r"(\w+): \[Tensor, Tensor, number, string\]\[\] =", r"\1 =", body)
+    body = re.sub(r"(\w+): (Float32Array|DevBuf|number|string)(\[\])? =", r"\1 =", body)
+    return re.sub(r"(?<=[\w\])])!(?=[.;,)\[])", "", body)
+
+
+def method(cls, name):
+    """(parameter names, plain body) of a method."""
+    at = SRC.index(f"export class {cls}")
+    m = re.compile(rf"^  (?:async |private )*{name}\(([^)]*)\)[^{{;]*?(?:: [^{{]*(?:\{{[^}}]*\}}[^{{]*)?)? \{{$", re.M).search(SRC, at)
+    params = [p.split(":")[0].strip(" ?") for p in m.group(1).split(",") if p.strip()]
+    return params, plain(block(SRC, m.end() - 1))
+
+
+def run(js):
+    out = subprocess.run(["node", "-e", js], capture_output=True, text=True, timeout=60)
+    assert out.returncode == 0, out.stderr[-2000:]
+    return json.loads(out.stdout)
+
+
+QK = """
+const prod = (s) => s.reduce((a, b) => a * b, 1);
+function backend() {
+  const log = [];
+  const be = {
+    log, ctx: "ctx", next: 100n,
+    sym: new Proxy({}, { get: (_, name) => (...a) => { log.push([name, a.slice(1).map(String)]); return 0; } }),
+    check(rc, what) { if (rc !== 0) throw new Error(what); },
+    dataOf(t) { return t.d || (t.d = be.next++); },
+    makeOut(shape, prev, alloc = true) { const t = { shape, _prev: prev, _backward() {} }, e = { data: alloc ? be.next++ : 0n, gradInit: false }; t.e = e; return { t, e }; },
+    gradOf(t) { t.e.gradInit = true; return t.g || (t.g = be.next++); },
+    gradDst(t) { const acc = t.acc || 0; t.acc = 1; return [t.gr || (t.gr = be.next++), acc]; },
+  };
+  be.qkNormRope = function (%s) %s;
+  return be;
+}
+const T = (...shape) => ({ shape, requiresGrad: true, _prev: [] });
+// the reference's walk: each tensor after everything below it, then backwards
+function walk(root) {
+  const seen = new Set(), topo = [];
+  (function go(t) { if (seen.has(t)) return; seen.add(t); t._prev.forEach(go); topo.push(t); })(root);
+  root.e.gradInit = true;
+  topo.reverse().forEach((t) => t._backward && t._backward());
+}
+"""
+
+
+def qk(js):
+    params, body = method("HipBackend", "qkNormRope")
+    return run(QK % (", ".join(params), body) + js)
+
+
+def tried(call):
+    return "(() => { const be = backend(); let err = ''; try { " + call + " } catch (e) { err = e.message; } return [err, be.log.map((x) => x[0])]; })()"
+
+
+@needs_node
+def test_qk_norm_rope_checks_its_shapes_before_it_calls():
+    """The library takes addresses: a row count or a width that is not what the tensors have would be read past their ends."""
+    cases = ["be.qkNormRope(T(6, 32), T(6, 16), T(8), T(8), 3, 4, 2, 8, 1e-6, 1e4, 0)",
+             "be.qkNormRope(T(6, 32), T(5, 16), T(8), T(8), 3, 4, 2, 8, 1e-6, 1e4, 0)",
+             "be.qkNormRope(T(6, 24), T(6, 16), T(8), T(8), 3, 4, 2, 8, 1e-6, 1e4, 0)",
+             "be.qkNormRope(T(6, 32), T(6, 16), T(8), T(7), 3, 4, 2, 8, 1e-6, 1e4, 0)",
+             "be.qkNormRope(T(6, 32), T(6, 8), T(8), T(8), 3, 4, 2, 8, 1e-6, 1e4, 0)",
+             "be.qkNormRope(T(6, 32), T(96), T(8), T(8), 3, 4, 2, 8, 1e-6, 1e4, 0)",
+             "const q = T(6, 16); be.qkNormRope(q, q, T(8), T(8), 3, 2, 2, 8, 1e-6, 1e4, 0)"]
+    got = qk("console.log(JSON.stringify([" + ", ".join(tried(c) for c in cases) + "]))")
+    assert got[0] == ["", ["gt_qk_norm_rope_fwd"]]
+    for (err, calls), match in zip(got[1:], ("6 rows and k 5", "q is [6, 24]", "gain of 7", "k is [6, 8]", "k is [96]", "distinct")):
+        assert match in err and calls == [], (err, match, calls)
