@@ -761,8 +761,9 @@ export class HipBackend implements OpsBackend, RegionBackend {
   }
 
   /** rope(rmsNormHeads(q)) and rope(rmsNormHeads(k)) as one launch each way (gt_qk_norm_rope_*), for a host whose layer bodies
-   * (src/arch/qwen3.ts, gemma3.ts) call it in place of the four ops. k's output names q's as its predecessor, so the closure
-   * on q's output runs when both gradients are complete. q and k, and their gains, must be distinct tensors. */
+   * (src/arch/qwen3.ts, gemma3.ts) call it in place of the four ops. The op is a node of its own behind its two outputs, so its closure
+   * runs when both gradients are complete. A walk visits the inputs of both whichever it came through: after one that came through an
+   * output, one that does not would hand that output's gradient on again, and is refused. q and k, and their gains, must be distinct tensors. */
   qkNormRope(
     q: Tensor, k: Tensor, qw: Tensor, kw: Tensor, T: number, Hq: number, Hkv: number, hd: number, eps: number, base: number,
     posOffset: number,
@@ -777,14 +778,28 @@ export class HipBackend implements OpsBackend, RegionBackend {
     if (q.shape[0] !== k.shape[0]) throw new Error(`qkNormRope: q has ${q.shape[0]} rows and k ${k.shape[0]}`);
     const rows = q.shape[0], ldq = BigInt(Hq * hd), ldk = BigInt(Hkv * hd);
     const qd = this.dataOf(q), kd = this.dataOf(k), qwd = this.dataOf(qw), kwd = this.dataOf(kw);
-    const { t: qo, e: eq } = this.makeOut([rows, Hq * hd], [q, k, qw, kw]);
-    const { t: ko, e: ek } = this.makeOut([rows, Hkv * hd], [qo]);
+    const { t: op } = this.makeOut([1], [q, k, qw, kw], false);
+    const { t: qo, e: eq } = this.makeOut([rows, Hq * hd], [op]);
+    const { t: ko, e: ek } = this.makeOut([rows, Hkv * hd], [op]);
     this.check(
       this.sym.gt_qk_norm_rope_fwd(this.ctx, rows, T, Hq, Hkv, hd, eps, base, posOffset, 0n, qd, ldq, qwd, eq.data, ldq, kd, ldk, kwd, ek.data, ldk),
       "qkNormRope",
     );
     const wantsQ = qw.requiresGrad, wantsK = kw.requiresGrad;
+    const now = [false, false], before = [false, false]; // the outputs that this walk, and an earlier one, came through
     qo._backward = () => {
+      now[0] = true;
+    };
+    ko._backward = () => {
+      now[1] = true;
+    };
+    op._backward = () => {
+      const missed = [0, 1].some((i) => before[i] && !now[i]);
+      for (const i of [0, 1]) {
+        before[i] = before[i] || now[i];
+        now[i] = false;
+      }
+      if (missed) throw new Error("qkNormRope: a backward reaches one output only, after one that reached the other: sync() between them");
       const gq = this.gradOf(qo), gk = this.gradOf(ko);
       const [dq, aq] = this.gradDst(q), [dk, ak] = this.gradDst(k);
       const [dwq, awq] = wantsQ ? this.gradDst(qw) : [0n, 0] as [DevBuf, number];

@@ -96,3 +96,27 @@ def test_qk_norm_rope_checks_its_shapes_before_it_calls():
     assert got[0] == ["", ["gt_qk_norm_rope_fwd"]]
     for (err, calls), match in zip(got[1:], ("6 rows and k 5", "q is [6, 24]", "gain of 7", "k is [6, 8]", "k is [96]", "distinct")):
         assert match in err and calls == [], (err, match, calls)
+
+
+@needs_node
+def test_qk_norm_rope_and_backwards_that_reach_one_output():
+    """Both outputs in one walk are one call; a walk through one output alone has zeros for the other; but where an earlier walk came through the other,
+    its old gradient would be handed on again: that is refused before anything is launched."""
+    js = """
+    const out = {};
+    for (const [name, walks] of Object.entries({ both: ["qk"], twice: ["qk", "qk"], q: ["q"], k: ["k"], qq: ["q", "q"], bothThenQ: ["qk", "q"], bothThenK: ["qk", "k"], kThenQ: ["k", "q"], qThenBoth: ["q", "qk"] })) {
+      const be = backend();
+      const [qo, ko] = be.qkNormRope(T(6, 32), T(6, 16), T(8), T(8), 3, 4, 2, 8, 1e-6, 1e4, 0);
+      let err = "";
+      try {
+        for (const w of walks) walk({ shape: [1], _prev: w === "qk" ? [qo, ko] : w === "q" ? [qo] : [ko], e: {} });
+      } catch (e) { err = e.message; }
+      out[name] = [err, be.log.filter((x) => x[0] === "gt_qk_norm_rope_bwd").length];
+    }
+    console.log(JSON.stringify(out));
+    """
+    got = qk(js)
+    for name, n in dict(both=1, twice=2, q=1, k=1, qq=2, qThenBoth=2).items():
+        assert got[name] == ["", n], (name, got[name])
+    for name in ("bothThenQ", "bothThenK", "kThenQ"):
+        assert "sync()" in got[name][0] and got[name][1] == 1, (name, got[name])
