@@ -1035,13 +1035,16 @@ export class AdamWHip {
     const m: Float32Array[] = [], v: Float32Array[] = [];
     if (this.opts.stateBits === 8) {
       const [bm, bv] = this.momentPair();
-      for (let i = 0; i < this.params.length; i++) {
-        this.gpu.check(this.gpu.symbols.gt_adamw8_read(this.gpu.context, this.handle, i, bm, bv), "gt_adamw8_read");
-        m.push(await this.gpu.readStateBuffer(bm, this.params[i].size));
-        v.push(await this.gpu.readStateBuffer(bv, this.params[i].size));
+      try {
+        for (let i = 0; i < this.params.length; i++) {
+          this.gpu.check(this.gpu.symbols.gt_adamw8_read(this.gpu.context, this.handle, i, bm, bv), "gt_adamw8_read");
+          m.push(await this.gpu.readStateBuffer(bm, this.params[i].size));
+          v.push(await this.gpu.readStateBuffer(bv, this.params[i].size));
+        }
+      } finally {
+        this.gpu.freeStateBuffer(bm);
+        this.gpu.freeStateBuffer(bv);
       }
-      this.gpu.freeStateBuffer(bm);
-      this.gpu.freeStateBuffer(bv);
       return { m, v, t: this.t };
     }
     for (let i = 0; i < this.params.length; i++) {
@@ -1061,13 +1064,16 @@ export class AdamWHip {
         }
       }
       const [bm, bv] = this.momentPair();
-      for (let i = 0; i < this.params.length; i++) {
-        this.gpu.writeStateBuffer(bm, s.m[i]);
-        this.gpu.writeStateBuffer(bv, s.v[i]);
-        this.gpu.check(this.gpu.symbols.gt_adamw8_write(this.gpu.context, this.handle, i, bm, bv), "gt_adamw8_write");
+      try {
+        for (let i = 0; i < this.params.length; i++) {
+          this.gpu.writeStateBuffer(bm, s.m[i]);
+          this.gpu.writeStateBuffer(bv, s.v[i]);
+          this.gpu.check(this.gpu.symbols.gt_adamw8_write(this.gpu.context, this.handle, i, bm, bv), "gt_adamw8_write");
+        }
+      } finally {
+        this.gpu.freeStateBuffer(bm);
+        this.gpu.freeStateBuffer(bv);
       }
-      this.gpu.freeStateBuffer(bm);
-      this.gpu.freeStateBuffer(bv);
       this.t = s.t;
       return;
     }

@@ -120,3 +120,67 @@ def test_qk_norm_rope_and_backwards_that_reach_one_output():
         assert got[name] == ["", n], (name, got[name])
     for name in ("bothThenQ", "bothThenK", "kThenQ"):
         assert "sync()" in got[name][0] and got[name][1] == 1, (name, got[name])
+
+
+# ---- AdamWHip -----------------------------------------------------------------------------------------------------------
+
+ADAM = """
+class Buffers {
+  // a backend that counts state buffers and fails at the n-th call of an entry point
+  constructor(fail, at) {
+    this.live = new Set(); this.n = 0; this.calls = []; this.context = null; this.isDestroyed = false;
+    let k = 0;
+    this.symbols = new Proxy({}, { get: (_, name) => (...a) => { this.calls.push(name); return name === fail && ++k === at ? 1 : 0; } });
+  }
+  check(rc, what) { if (rc !== 0) throw new Error(what); }
+  createStateBuffer(bytes) { const b = BigInt(++this.n); this.live.add(b); return b; }
+  freeStateBuffer(b) { this.live.delete(b); }
+  writeStateBuffer() { if (--this.writes === 0) throw new Error("write"); }
+  async readStateBuffer(b, n) { if (--this.reads === 0) throw new Error("read"); return new Float32Array(n); }
+  buffersFor() { return { data: 1n, grad: 2n }; }
+  keepGradOnDevice() {}
+}
+const Deno = { UnsafePointer: { create: (x) => x } }, u64s = (v) => v;
+class AdamWHip {
+  %s
+}
+const P = (n) => ({ size: n });
+const S = (...n) => n.map((k) => new Float32Array(k));
+async function main() { const out = []; %s; console.log(JSON.stringify(out)); }
+main().catch((e) => { console.error(e); process.exit(1); });
+"""
+
+
+def adam(js):
+    names = ("constructor", "momentPair", "exportState", "importState", "destroy")
+    body = []
+    for n in names:
+        at = SRC.index("export class AdamWHip")
+        m = re.compile(rf"^  ((?:async |private )*){n}\((.*)\)(?:: .*)? \{{$", re.M).search(SRC, at)
+        params = [re.sub(r"\W", "", p.split(":")[0]) for p in re.split(r",(?![^{]*\})", m.group(2)) if p.strip()]
+        fields = "this.mBufs = []; this.vBufs = []; this.eBufs = []; this.t = 0; this.handle = null;" if n == "constructor" else ""
+        text = plain(block(SRC, m.end() - 1))
+        body.append(f"{'async ' if 'async' in m.group(1) else ''}{n}({', '.join(params)}) {{ {fields}" + text[1:])
+    return run(ADAM % ("\n".join(body), js))
+
+
+@needs_node
+@pytest.mark.parametrize("bits", [8, 32])
+def test_adamw_gives_its_moment_buffers_back_when_a_call_throws(bits):
+    """However far exportState and importState come, the state buffers afterwards are those of the group."""
+    js = """
+    for (const [what, fail, at] of [["", "", 0], ["export", "gt_adamw8_read", 2], ["exportRead", "", 3], ["import", "gt_adamw8_write", 2], ["importWrite", "", 3]]) {
+      const gpu = new Buffers(fail, at), opt = new AdamWHip(gpu, [P(300), P(5)], { lr: 1, stateBits: %d });
+      const own = gpu.live.size;
+      gpu.reads = what === "exportRead" ? at : -1;
+      gpu.writes = what === "importWrite" ? at : -1;
+      let err = "";
+      try { const s = await opt.exportState(); opt.importState({ m: S(300, 5), v: S(300, 5), t: 3 }); } catch (e) { err = e.message; }
+      out.push([what, err, own, gpu.live.size]);
+      opt.destroy();
+      out.push(gpu.live.size);
+    }""" % bits
+    got = adam(js)
+    for done, rest in zip(got[::2], got[1::2]):
+        assert done[2] == done[3] == (6 if bits == 8 else 4) and rest == 0, done
+        assert bool(done[1]) == (done[0] != "" and (bits == 8 or done[0] in ("exportRead", "importWrite"))), done
