@@ -967,7 +967,8 @@ export class AdamWHip {
   constructor(gpu: HipBackend, params: Tensor[], opts: AdamHipOpts) {
     this.gpu = gpu;
     this.params = params;
-    this.opts = { beta1: 0.9, beta2: 0.999, eps: 1e-8, weightDecay: 0.0, clip: 1.0, stateBits: 32, ...opts };
+    this.opts = { beta1: 0.9, beta2: 0.999, eps: 1e-8, weightDecay: 0.0, clip: 1.0, ...opts, stateBits: opts.stateBits ?? 32 };
+    if (this.opts.stateBits !== 8 && this.opts.stateBits !== 32) throw new Error(`AdamW: stateBits must be 8 or 32, got ${this.opts.stateBits}`);
     this.baseLr = opts.lr;
     const per = this.opts.stateBits === 8 ? 1 : 4;
     const w: DevBuf[] = [], g: DevBuf[] = [];

@@ -184,3 +184,19 @@ def test_adamw_gives_its_moment_buffers_back_when_a_call_throws(bits):
     for done, rest in zip(got[::2], got[1::2]):
         assert done[2] == done[3] == (6 if bits == 8 else 4) and rest == 0, done
         assert bool(done[1]) == (done[0] != "" and (bits == 8 or done[0] in ("exportRead", "importWrite"))), done
+
+
+@needs_node
+def test_adamw_refuses_other_state_sizes():
+    js = """
+    for (const bits of [16, 0, "8", 8, 32, undefined]) {
+      const gpu = new Buffers("", 1);
+      let err = "";
+      try { new AdamWHip(gpu, [P(300)], { lr: 1, stateBits: bits }); } catch (e) { err = e.message; }
+      out.push([err, gpu.live.size, gpu.calls]);
+    }"""
+    got = adam(js)
+    for err, live, calls in got[:3]:
+        assert "stateBits must be 8 or 32" in err and live == 0 and calls == []
+    for (err, live, calls), (n, name) in zip(got[3:], ((3, "gt_adamw8_create"), (2, "gt_adamw_create"), (2, "gt_adamw_create"))):
+        assert err == "" and live == n and calls == [name]
