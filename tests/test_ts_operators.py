@@ -29,6 +29,7 @@ def plain(body):
     body = re.sub(r"\bas (\[[^\]]*\]|\w+)(\[\])?", "", body)
     body = re.sub(r"(\w+): \[Tensor, Tensor, number, string\]\[\] =", r"\1 =", body)
     body = re.sub(r"(\w+): (Float32Array|DevBuf|number|string)(\[\])? =", r"\1 =", body)
+    body = re.sub(r"([\w.]+) \?\? (\w+)", r"(\1 != null ? \1 : \2)", body)       # younger than the node this may meet
     return re.sub(r"(?<=[\w\])])!(?=[.;,)\[])", "", body)
 
 
