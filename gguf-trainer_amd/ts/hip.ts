@@ -970,34 +970,39 @@ export class AdamWHip {
     this.opts = { beta1: 0.9, beta2: 0.999, eps: 1e-8, weightDecay: 0.0, clip: 1.0, ...opts, stateBits: opts.stateBits ?? 32 };
     if (this.opts.stateBits !== 8 && this.opts.stateBits !== 32) throw new Error(`AdamW: stateBits must be 8 or 32, got ${this.opts.stateBits}`);
     this.baseLr = opts.lr;
-    const per = this.opts.stateBits === 8 ? 1 : 4;
-    const w: DevBuf[] = [], g: DevBuf[] = [];
-    for (const p of params) {
-      const b = gpu.buffersFor(p); // uploads host weights once; accumulator on the device
-      gpu.keepGradOnDevice(p);
-      w.push(b.data);
-      g.push(b.grad);
-      this.mBufs.push(gpu.createStateBuffer(p.size * per));
-      this.vBufs.push(gpu.createStateBuffer(p.size * per));
-      if (this.opts.stateBits === 8) this.eBufs.push(gpu.createStateBuffer(2 * Math.ceil(p.size / 256)));
+    try {
+      const per = this.opts.stateBits === 8 ? 1 : 4;
+      const w: DevBuf[] = [], g: DevBuf[] = [];
+      for (const p of params) {
+        const b = gpu.buffersFor(p); // uploads host weights once; accumulator on the device
+        gpu.keepGradOnDevice(p);
+        w.push(b.data);
+        g.push(b.grad);
+        this.mBufs.push(gpu.createStateBuffer(p.size * per));
+        this.vBufs.push(gpu.createStateBuffer(p.size * per));
+        if (this.opts.stateBits === 8) this.eBufs.push(gpu.createStateBuffer(2 * Math.ceil(p.size / 256)));
+      }
+      const sizes = BigInt64Array.from(params.length ? params.map((p) => BigInt(p.size)) : [0n]);
+      const out = new BigUint64Array(1);
+      const o = this.opts;
+      if (o.stateBits === 8) {
+        gpu.check(
+          gpu.symbols.gt_adamw8_create(gpu.context, params.length, u64s(w), u64s(g), u64s(this.mBufs), u64s(this.vBufs), u64s(this.eBufs),
+            sizes, o.beta1, o.beta2, o.eps, o.weightDecay, o.clip, out),
+          "gt_adamw8_create",
+        );
+      } else {
+        gpu.check(
+          gpu.symbols.gt_adamw_create(gpu.context, params.length, u64s(w), u64s(g), u64s(this.mBufs), u64s(this.vBufs), sizes,
+            o.beta1, o.beta2, o.eps, o.weightDecay, o.clip, out),
+          "gt_adamw_create",
+        );
+      }
+      this.handle = Deno.UnsafePointer.create(out[0]);
+    } catch (e) {
+      this.destroy(); // a refused group keeps no memory
+      throw e;
     }
-    const sizes = BigInt64Array.from(params.length ? params.map((p) => BigInt(p.size)) : [0n]);
-    const out = new BigUint64Array(1);
-    const o = this.opts;
-    if (o.stateBits === 8) {
-      gpu.check(
-        gpu.symbols.gt_adamw8_create(gpu.context, params.length, u64s(w), u64s(g), u64s(this.mBufs), u64s(this.vBufs), u64s(this.eBufs),
-          sizes, o.beta1, o.beta2, o.eps, o.weightDecay, o.clip, out),
-        "gt_adamw8_create",
-      );
-    } else {
-      gpu.check(
-        gpu.symbols.gt_adamw_create(gpu.context, params.length, u64s(w), u64s(g), u64s(this.mBufs), u64s(this.vBufs), sizes,
-          o.beta1, o.beta2, o.eps, o.weightDecay, o.clip, out),
-        "gt_adamw_create",
-      );
-    }
-    this.handle = Deno.UnsafePointer.create(out[0]);
   }
   setLrScale(scale: number) {
     this.lrScale = scale;

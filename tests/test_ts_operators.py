@@ -201,3 +201,15 @@ def test_adamw_refuses_other_state_sizes():
         assert "stateBits must be 8 or 32" in err and live == 0 and calls == []
     for (err, live, calls), (n, name) in zip(got[3:], ((3, "gt_adamw8_create"), (2, "gt_adamw_create"), (2, "gt_adamw_create"))):
         assert err == "" and live == n and calls == [name]
+
+
+@needs_node
+def test_a_refused_adamw_group_keeps_no_memory():
+    js = """
+    for (const [bits, fail] of [[8, "gt_adamw8_create"], [32, "gt_adamw_create"]]) {
+      const gpu = new Buffers(fail, 1);
+      let err = "";
+      try { new AdamWHip(gpu, [P(300), P(5)], { lr: 1, stateBits: bits }); } catch (e) { err = e.message; }
+      out.push([err, gpu.n, gpu.live.size]);
+    }"""
+    assert adam(js) == [["gt_adamw8_create", 6, 0], ["gt_adamw_create", 4, 0]]
