@@ -20,7 +20,7 @@
 //
 // Bound by memory: 16 bytes per element (g read, w read and written, two codes each way), 20 with the clip, whose norm has
 // to be known before the first update. One wavefront to a block, four neighbouring elements to a lane, so that the block's
-// largest moments are one exchange within the wavefront and no LDS is used. About 60 vector operations per element: at
+// largest moments are one exchange within the wavefront and no LDS is used. 63 vector operations per element: at
 // twice that (library roots and divisions, float comparisons for the block's largest) they were as long as the memory's time.
 #include <algorithm>
 #include <exception>
@@ -46,7 +46,8 @@ typedef GLOBAL unsigned char gbyte;
 
 struct Adam8H { float b1, b2, omb1, omb2, eps, wd, lr, ibc1, rbc2; unsigned key; };
 
-// The random bits: a multiply-xorshift mixer, two rounds of it for a block's key and one from there for each element.
+// The random bits: a multiply-xorshift mixer (shifts 16, 15, 15 and two factors published with the hash-prospector search, public domain), two
+// rounds of it for a block's key and one from there for each element.
 __host__ __device__ __forceinline__ unsigned mix1(unsigned x) {
   x ^= x >> 16;
   x *= 0x21F0AAADu;

@@ -951,7 +951,8 @@ export interface AdamHipOpts extends AdamOpts {
 }
 
 /** AdamWGpu (adamw-gpu.ts:131-251) over gt_adamw_*: weights, gradients and moments stay on the device; a step is three
- * launches for any number of tensors (sum of squares, clip scale, fused update; two with 8-bit moments). */
+ * launches for any number of tensors (sum of squares, clip scale, fused update). With 8-bit moments it is one without a clip, two with one up to
+ * two million parameters or so (2048 chunks of 1024), three beyond. */
 export class AdamWHip {
   readonly params: Tensor[];
   private gpu: HipBackend;

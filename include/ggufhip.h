@@ -334,17 +334,17 @@ int gt_adamw_destroy(gt_ctx *ctx, gt_adamw *opt);
 /* The same step with the moments held in 8 bits: 2 bytes of state per parameter instead of 8, 16 (20 with the clip) bytes moved per
  * parameter and step instead of 28 (32). No counterpart in the reference. m[i] and r[i] are sizes[i] bytes each: the first moment
  * and the ROOT of the second as OCP e4m3 values; e[i] holds two signed bytes for each block of 256 elements (2 * ceil(sizes[i] / 256)
- * bytes, 2-byte aligned), the exponents of m (-126 or more) and of r (-65 or more; -126 in a block of zeros): a state is its e4m3 value times 2^e. All bytes zero = zero moments. The
- * caller owns and clears the buffers. Each step rounds the new moments up or down at random in proportion, from bits that `seed`,
- * the block and the place in it determine: pass another seed each step (the step number will do); the same seed gives the
- * same bits. Gradients and weights are FP32, the update uses the moments before they are rounded, and the norm for the
- * clip is summed in 64 bits. A moment that is not finite is held as e4m3's NaN; of r
- * the positive one stands for infinity (a square that left FP32: its weight is left to its decay, as by gt_adamw_step), the negative one
- * for NaN. The handle is gt_adamw's: gt_adamw_grad_norm and
- * gt_adamw_destroy take it, gt_adamw_step does not. A step allocates nothing. No two of the w, m, r and e buffers may overlap, and no
- * gradient may overlap one of them.
+ * bytes, 2-byte aligned), the exponents of m (-126 or more) and of r (-65 or more, so that every r^2 is an FP32 number; -126 in a block of
+ * zeros): a state is its e4m3 value times 2^e. All bytes zero = zero moments. The caller owns and clears the buffers. Each step rounds
+ * the new moments up or down at random in proportion, from bits that `seed`, the block and the place in it determine: pass another seed each
+ * step (the step number will do); the same seed gives the same bits. Gradients and weights are FP32, the update uses the moments before
+ * they are rounded, and the norm for the clip is summed in 64 bits. A moment that is not finite is held as e4m3's NaN; of r the positive one
+ * stands for infinity (a square that left FP32: its weight is left to its decay, as by gt_adamw_step), the negative one for NaN. The
+ * handle is gt_adamw's: gt_adamw_grad_norm and gt_adamw_destroy take it, gt_adamw_step does not. A step allocates nothing. No two of the
+ * w, m, r and e buffers may overlap, and no gradient may overlap one of them.
  *   gt_adamw8_read:  the moments of tensor i as FP32 values, m and v = r^2 (0: not wanted)
- *   gt_adamw8_write: the states of tensor i from FP32 moments, rounded to nearest; what gt_adamw8_read gave comes back unchanged */
+ *   gt_adamw8_write: the states of tensor i from FP32 moments, rounded to nearest; what gt_adamw8_read gave comes back unchanged.
+ *                    Neither takes buffers that overlap the tensor's states, nor gt_adamw8_read two that overlap each other */
 int gt_adamw8_create(gt_ctx *ctx, int n, const gt_buf *w, const gt_buf *g, const gt_buf *m, const gt_buf *r, const gt_buf *e,
                      const int64_t *sizes, double beta1, double beta2, double eps, double weight_decay, double clip,
                      gt_adamw **out);
