@@ -1152,7 +1152,7 @@ class HipBackend:
             for t in (a, b):
                 te = self._entries.get(t)
                 if (self.alias_add_grads and te is not None and not te.external and not te.keep_grad and not te.grad_init
-                        and not te.grad_src and id(t) not in self._pend_dx):
+                        and not te.grad_src and not te.rope_fused and id(t) not in self._pend_dx):
                     te.grad_src = g             # first writer: the gradient IS the upstream one so far, nothing to launch
                     te.grad_init = True
                     self._aliased.append(t)

@@ -119,3 +119,14 @@ def test_an_output_that_is_gone_needs_no_gradient(gpu):
         out = ag.add(ag.scale(q0, 0.25), ag.scale(k0, 0.5))
         backward_from(gpu, ag, out, rs.standard_normal(out.size))
     both(gpu, body, 56)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["both", "q", "twice"])
+def test_a_sum_recorded_after_a_backward(gpu, which):
+    """An add hands its upstream gradient on by address where nobody has written one yet."""
+    def body(ag, rs, t, q, k, *_):
+        backward_from(gpu, ag, ag.attention(q, k, t["v"], T, H, H, HD), rs.standard_normal(T * H * HD))
+        out = ag.add(q, {"both": k, "q": t["v"], "twice": q}[which])
+        backward_from(gpu, ag, ag.scale(out, 0.5), rs.standard_normal(out.size))
+    both(gpu, body, 57)
