@@ -199,6 +199,7 @@ class HipBackend:
         # before any buffer they point at can be recycled.
         self.alias_add_grads = True
         self._aliased: list = []
+        self._lent: set = set()           # gradient buffers that a tensor of that list points at
         self.batch_linears = True
         # attention keeps its scores from the forward to the backward (one [T, T] matrix per sequence and head) when a
         # gradient will be asked for, one call's matrices fit attn_scores_max_bytes and the live ones together stay
@@ -601,6 +602,17 @@ class HipBackend:
         check(self._ctx, lib.gt_rope(self._ctx, t.shape[0], T, t.shape[1] // hd, hd, base, pos, 0, se.grad, e.grad, 0), "rope")
         e.grad_init = True
 
+    def _settle_lent(self, b: int):
+        """Gradient buffer b is about to change, which only a later backward over the same graph does: those who were handed its contents keep them."""
+        self._lent.discard(b)
+        for t in self._aliased:
+            e = self._entries.get(t)
+            if e is not None and e.grad_src == b:
+                if e.grad == 0:
+                    e.grad = self._acquire(e.nbytes, e.stream)
+                check(self._ctx, lib.gt_d2d(self._ctx, e.grad, b, e.nbytes), "gt_d2d")
+                e.grad_src = 0
+
     def _settle_rotated(self, e: _Entry):
         """The gradient of a rotation's input is about to be written by somebody else."""
         t, e.rope_out = e.rope_out, None
@@ -642,6 +654,8 @@ class HipBackend:
             return slot[0], acc
         if e.grad == 0:
             e.grad = self._acquire(e.nbytes, e.stream)
+        elif e.grad in self._lent:
+            self._settle_lent(e.grad)
         if e.grad_src:
             check(self._ctx, lib.gt_d2d(self._ctx, e.grad, e.grad_src, e.nbytes), "gt_d2d")
             e.grad_src = 0
@@ -692,6 +706,7 @@ class HipBackend:
                 check(self._ctx, lib.gt_d2d(self._ctx, e.grad, e.grad_src, e.nbytes), "gt_d2d")
                 e.grad_src = 0
         self._aliased = []
+        self._lent = set()
 
     def _gsrc(self, t: Tensor, unrotated: bool = False) -> int:
         """Gradient buffer of an op output inside its backward closure. unrotated: the closure looks at the entry's grad_unrotated and
@@ -824,6 +839,8 @@ class HipBackend:
                 se.rope_out = None
         if e.grad == 0:
             e.grad = self._acquire(e.nbytes, e.stream)
+        elif e.grad in self._lent:
+            self._settle_lent(e.grad)
         check(self._ctx, lib.gt_h2d(self._ctx, e.grad, t.grad.ctypes.data_as(C.c_void_p), e.nbytes), "gt_h2d")
         e.grad_init = True
         e.grad_src = 0
@@ -1156,6 +1173,7 @@ class HipBackend:
                     te.grad_src = g             # first writer: the gradient IS the upstream one so far, nothing to launch
                     te.grad_init = True
                     self._aliased.append(t)
+                    self._lent.add(g)
                 else:
                     todo.append(t)
             if len(todo) == 2:
